@@ -15,6 +15,7 @@ F32, BF16 = 0, 1
 MODE_AUTO = -1
 UP_CODES = {"coop": 0, "lane": 1, "tile": 2}
 DOWN_CODES = {"coop": 0, "tiled": 1, "blocked": 2}
+REDUCE_CODES = {"none": 0, "mean": 1, "sum": 2}
 
 _P = ctypes.c_void_p
 _I32, _I64 = ctypes.c_int32, ctypes.c_int64
@@ -103,6 +104,16 @@ SIGNATURES = {
                                           _I64, _P]),
     "hffn_forward_noalloc_max_bytes": (_I64, []),
     "hffn_forward_noalloc": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(Layer), _P, _P, _I64, _P]),
+    "hffn_linear_ce_state_bytes": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
+    "hffn_linear_ce_forward_workspace": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
+    "hffn_linear_ce_forward": (ctypes.c_int, [ctypes.c_int, _P, _I64, _P, _P, _I64, ctypes.c_int, _P, _P, _P, _I64,
+                                              _I32, _I32, _P]),
+    "hffn_linear_ce_backward_workspace": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
+    "hffn_linear_ce_backward": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P, _P, _P, _P, _P, _I64, _I32, _I32,
+                                               _P]),
+    "hffn_grad_norm_workspace": (_I64, [_I32]),
+    "hffn_grad_norm": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, _P]),
+    "hffn_clip_grad_norm": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, _P]),
     "hffn_densify_f16x3": (ctypes.c_int, [_P, _P, _P, _P, _I32, _I32, _P, _P, _P, _P, _P]),
     "hffn_forward_f16x3_workspace": (_I64, [ctypes.POINTER(Layer), _I64]),
     "hffn_forward_f16x3": (ctypes.c_int, [ctypes.POINTER(Layer), ctypes.POINTER(DenseF16x3), _P, _P, _P, _P, _P, _I64,

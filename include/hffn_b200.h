@@ -356,6 +356,48 @@ int hffn_train_step_tc(const hffn_layer* layer, const hffn_dense* dense, const h
                        const hffn_adamw_step* adamw, float* loss, void* work, int32_t* err, int64_t n, int64_t n_total,
                        void* stream);
 
+/* Reductions of hffn_linear_ce_forward. */
+#define HFFN_REDUCE_NONE 0
+#define HFFN_REDUCE_MEAN 1
+#define HFFN_REDUCE_SUM 2
+
+/* Linear softmax cross entropy of a language model's head (no counterpart in the reference, whose training step takes
+ * gy from the caller): hidden [n, d] (rows hidden_stride apart), weight [vocab, d], both of `dtype`, targets [n] (int64).
+ *   z_tv = hidden_t . weight_v,   loss_t = log sum_v exp z_tv - z_{t, target_t}
+ * The logits are never stored. A row whose target is ignore_index has loss 0 and takes no part; its hidden state is not
+ * read into any sum. A row whose target is otherwise outside [0, vocab) has loss NaN and no gradient. reduction NONE:
+ * loss [n] float32; MEAN: *loss = the sum over the kept rows / max(1, kept rows); SUM. d: a multiple of 8.
+ * state: hffn_linear_ce_state_bytes, kept for the backward; work: hffn_linear_ce_forward_workspace bytes (16-byte
+ * aligned, as weight). */
+int64_t hffn_linear_ce_state_bytes(int dtype, int64_t n, int32_t d, int32_t vocab);
+int64_t hffn_linear_ce_forward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab);
+int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
+                           const int64_t* targets, int64_t ignore_index, int reduction, float* loss, void* state,
+                           void* work, int64_t n, int32_t d, int32_t vocab, void* stream);
+
+/* The gradients of that forward (its state, the same weight): grad_hidden [n, d] and grad_weight [vocab, d] of `dtype`,
+ * contiguous, either NULL when it is not wanted. grad_loss: the loss's own gradient, float32 on the device: [n] for
+ * NONE, else one value. work: hffn_linear_ce_backward_workspace bytes. The logits are recomputed one piece of the
+ * vocabulary at a time. */
+int64_t hffn_linear_ce_backward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab);
+int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const float* grad_loss, void* grad_hidden,
+                            void* grad_weight, void* state, void* work, int64_t n, int32_t d, int32_t vocab,
+                            void* stream);
+
+/* The 2-norm over every entry of `count` tensors (no counterpart in the reference): tensors[i] holds numel[i] entries of
+ * dtypes[i] (the lists are host arrays, read before the call returns), summed in float64; *norm: float32 on the
+ * device. work: hffn_grad_norm_workspace bytes, 8-byte aligned. */
+int64_t hffn_grad_norm_workspace(int32_t count);
+int hffn_grad_norm(int32_t count, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, float* norm,
+                   void* work, void* stream);
+
+/* Clipping by that norm: outs[i] (numel[i] entries of out_dtypes[i]; outs[i] == tensors[i]: in place) = tensors[i] *
+ * min(1, max_norm / (norm + 1e-6)), in float32 and rounded once; *norm is the norm before it. Outputs that share memory
+ * with one another or with another tensor are refused. */
+int hffn_clip_grad_norm(int32_t count, const void* const* tensors, void* const* outs, const int64_t* numel,
+                        const int32_t* dtypes, const int32_t* out_dtypes, float max_norm, float* norm, void* work,
+                        void* stream);
+
 /* Forward that allocates nothing and needs no workspace from the caller. No counterpart in the reference.
  * Some callers can hand this library only their input and output buffers: a plugin whose host framework owns every
  * device allocation and exposes no allocator, or a caller that must not call cudaMalloc on its path (it can

@@ -1,0 +1,421 @@
+"""GPU: the linear softmax cross entropy (``hffn_b200.losses``) against its definition in float64.
+
+Every bound is elementwise and derived, not fitted. Notation: u = 2^-24 (half a step of float32), r the half step of
+the storage type (bfloat16 2^-8; float32: the operands of the products are held as two fp16 parts, whose
+representation and dropped low-by-low product are within r = 2^-20 of a product, then rounded once to float32).
+- A product summed over k terms in float32 is within acc(k) = (k / 16 + 32) 2^-23 of the sum of its terms' absolute
+  values (the tensor core adds 16 products at a time and truncates; one step each, and the sums within one add).
+- A logit is within dz = (acc(d) + [float32: r]) sum_i |h_i w_i| of the exact one; every exponential's argument and the log sum
+  are within the largest dz of a row plus rounding of a value of size |z|: e_t = 2 max_v dz + 8 u (max |z| + 1 + log V).
+- loss_t is within e_t + u (|lse| + |z|).
+- g = c (p - [target]) is within |c| p (e^{e_t} - 1 + 2^-20) + r |g| (its storage) of the exact one, and a gradient
+  sum_k g x is within sum_k |delta g| |x| + (acc(k) + [float32: r]) sum_k |g x| + r |result|.
+- Two fp16 parts hold an entry of float32 operands (hidden states, head, c h and p - [target]) to 2^-39 of the largest
+  entry of its operand at worst (the end of fp16's range), which adds that much per entry to every product.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+IGNORE = -100
+
+
+def make(n, d, v, dtype, seed=0, ignored=0.0, scale=2.0, ignore_index=IGNORE):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = (torch.randn(v, d, generator=g, device="cuda") * scale / math.sqrt(d)).to(dtype)
+    targets = torch.randint(0, v, (n,), generator=g, device="cuda")
+    lean = torch.rand(n, 1, generator=g, device="cuda") * 3
+    h = (torch.randn(n, d, generator=g, device="cuda") + lean * w[targets].float()).to(dtype)
+    if ignored:
+        targets[torch.rand(n, generator=g, device="cuda") < ignored] = ignore_index
+    return h, w, targets
+
+
+def acc(k):
+    return (k / 16 + 32) * 2.0 ** -23
+
+
+def reference(h, w, targets, c, ignore_index=IGNORE):
+    """Losses and both gradients in float64 for upstream gradients ``c`` [n] (0 where ignored), and their bounds."""
+    fp32 = h.dtype == torch.float32
+    store = 2.0 ** -20 if fp32 else 2.0 ** -8
+    split = 2.0 ** -20 if fp32 else 0.0
+    out_r = U if fp32 else 2.0 ** -8
+    n, d = h.shape
+    v = w.shape[0]
+    keep = targets != ignore_index
+    h64 = torch.where(keep[:, None], h, torch.zeros_like(h)).double()
+    w64 = w.double()
+    z = h64 @ w64.T
+    held = 2.0 ** -39 if fp32 else 0.0          # of the largest entry of an operand
+    h_held, w_held = held * h64.abs().amax(), held * w64.abs().amax()
+    dz = (acc(d) + split) * (h64.abs() @ w64.abs().T).amax(1) + h_held * w64.abs().sum(1).amax() \
+        + w_held * h64.abs().sum(1)
+    lse = torch.logsumexp(z, 1)
+    picked = z.gather(1, targets.clamp(min=0)[:, None]).squeeze(1)
+    losses = torch.where(keep, lse - picked, 0.0)
+    e = 2 * dz + 8 * U * (z.abs().amax(1) + 1 + math.log(v))
+    loss_bound = torch.where(keep, e + 2 * U * (lse.abs() + picked.abs()), 0.0)
+    p = (z - lse[:, None]).exp()
+    g = p.clone()
+    g.scatter_add_(1, targets.clamp(min=0)[:, None], torch.full((n, 1), -1.0, dtype=torch.float64, device="cuda"))
+    c64 = torch.where(keep, c.double(), 0.0)
+    g = g * c64[:, None]
+    dg = c64.abs()[:, None] * ((torch.expm1(e) + 2.0 ** -20)[:, None] * p + held) + (store + 4 * U) * g.abs()
+    dg = torch.where(keep[:, None], dg, 0.0)
+    dh, dw = g @ w64, g.T @ h64
+    k_n = max(1, int(keep.sum()))
+    dh_bound = dg @ w64.abs() + (acc(v) + split) * (g.abs() @ w64.abs()) + out_r * dh.abs()
+    dh_bound += w_held * g.abs().sum(1, keepdim=True)
+    dw_bound = dg.T @ h64.abs() + (acc(k_n) + split) * (g.abs().T @ h64.abs()) + out_r * dw.abs()
+    ch = held * (c64[:, None] * h64).abs().amax()
+    unit = torch.where(c64 == 0, 0.0, 1 / torch.where(c64 == 0, 1.0, c64.abs()))
+    dw_bound += ch * (g.abs() * unit[:, None]).sum(0)[:, None]
+    return (losses, loss_bound), (dh, 1.01 * dh_bound + 1e-30), (dw, 1.01 * dw_bound + 1e-30)
+
+
+def within(actual, expected, what):
+    value, bound = expected
+    assert actual.shape == value.shape, what
+    off = (actual.double() - value).abs()
+    assert bool(torch.isfinite(actual).all()), what
+    worst = (off / (bound + 1e-300)).max()
+    assert bool((off <= bound).all()), f"{what}: {float(worst)} of the bound, off by {float(off.max())}"
+
+
+def check(h, w, targets, reduction="none", seed=3, ignore_index=IGNORE):
+    from hffn_b200.losses import linear_cross_entropy
+    n = h.shape[0]
+    kept = max(1, int((targets != ignore_index).sum()))
+    if reduction == "none":
+        c = torch.randn(n, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+    else:
+        c = torch.full((n,), 1.0 / kept if reduction == "mean" else 1.0, dtype=torch.float64, device="cuda")
+    expected_losses, expected_dh, expected_dw = reference(h, w, targets, c, ignore_index)
+    h, w = h.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    loss = linear_cross_entropy(h, w, targets, ignore_index=ignore_index, reduction=reduction)
+    assert loss.dtype == torch.float32
+    dh, dw = torch.autograd.grad(loss, (h, w), c if reduction == "none" else None)
+    assert dh.dtype == h.dtype and dw.dtype == w.dtype
+    if reduction == "none":
+        within(loss.detach(), expected_losses, "losses")
+    else:
+        share = kept if reduction == "mean" else 1
+        total, bound = expected_losses[0].sum() / share, expected_losses[1].sum() / share
+        within(loss.detach(), (total, bound + U * total.abs()), "loss")
+    within(dh, expected_dh, "grad_hidden")
+    within(dw, expected_dw, "grad_weight")
+    return loss.detach(), dh, dw
+
+
+BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+SHAPES = [(1, 8, 1), (1, 64, 2), (2, 72, 7), (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
+          (256, 512, 1000), (257, 1024, 2049), (700, 328, 4099), (1, 1024, 50304), (9, 2048, 5001), (1021, 768, 3001)]
+
+
+@BOTH
+@pytest.mark.parametrize("n,d,v", SHAPES)
+def test_against_float64(n, d, v, dtype):
+    check(*make(n, d, v, dtype, seed=n + v))
+
+
+@BOTH
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("ignored", [0.0, 0.3])
+def test_reductions(reduction, ignored, dtype):
+    check(*make(190, 128, 1500, dtype, seed=5, ignored=ignored), reduction=reduction)
+
+
+@BOTH
+@pytest.mark.parametrize("ignored", [0.1, 0.9])
+@pytest.mark.parametrize("n", [3, 256, 515])
+def test_ignored_rows(n, ignored, dtype):
+    h, w, t = make(n, 96, 777, dtype, seed=n, ignored=ignored)
+    t[0] = IGNORE
+    losses, dh, _ = check(h, w, t)
+    gone = t == IGNORE
+    assert bool((losses[gone] == 0).all()) and bool((dh[gone] == 0).all())
+
+
+@BOTH
+def test_several_pieces_of_the_vocabulary(dtype):
+    """Enough tokens that g is held in several pieces (float32: from 1334 tokens of 50304 ids)."""
+    check(*make(6200, 64, 50304, dtype, seed=8, ignored=0.05), reduction="mean")
+
+
+@BOTH
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+def test_every_row_ignored(reduction, dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(300, 64, 500, dtype)
+    h[:] = float("nan")
+    t[:] = IGNORE
+    h.requires_grad_(True), w.requires_grad_(True)
+    loss = linear_cross_entropy(h, w, t, reduction=reduction)
+    dh, dw = torch.autograd.grad(loss.sum(), (h, w))
+    for x in (loss, dh, dw):
+        assert bool((x == 0).all())
+
+
+@BOTH
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+def test_what_ignored_rows_hold_reaches_nothing(poison, dtype):
+    h, w, t = make(333, 72, 900, dtype, seed=2, ignored=0.4)
+    clean = check(h, w, t)
+    h = h.clone()
+    h[t == IGNORE] = poison
+    dirty = check(h, w, t)
+    for a, b in zip(clean, dirty):
+        assert torch.equal(a, b)
+
+
+@BOTH
+def test_a_row_that_is_not_finite_stays_alone(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(40, 64, 300, dtype, seed=4)
+    h = h.clone()
+    h[7, 3] = float("nan")
+    h[20, 0] = float("inf")
+    h.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    (dh,) = torch.autograd.grad(losses.sum(), h)
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[7, 20]] = True
+    assert not bool(torch.isfinite(losses[bad]).any())
+    assert bool(torch.isfinite(losses[~bad]).all()) and bool(torch.isfinite(dh[~bad]).all())
+    expected = reference(h.detach()[~bad], w, t[~bad], torch.ones(38, device="cuda"))
+    within(losses.detach()[~bad], expected[0], "losses")
+    within(dh[~bad], expected[1], "grad_hidden")
+
+
+@BOTH
+def test_targets_out_of_range_give_nan_and_no_gradient(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(50, 64, 300, dtype, seed=6)
+    t[3], t[11], t[49] = 300, -1, 2 ** 40
+    bad = torch.zeros(50, dtype=torch.bool, device="cuda")
+    bad[[3, 11, 49]] = True
+    h.requires_grad_(True), w.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    dh, dw = torch.autograd.grad(losses, (h, w), torch.ones_like(losses))
+    assert bool(torch.isnan(losses[bad]).all()) and bool((dh[bad] == 0).all())
+    expected = reference(h.detach()[~bad], w.detach(), t[~bad], torch.ones(47, device="cuda"))
+    within(losses.detach()[~bad], expected[0], "losses")
+    within(dh[~bad], expected[1], "grad_hidden")
+    within(dw, expected[2], "grad_weight")
+    assert bool(torch.isnan(linear_cross_entropy(h, w, t)))
+
+
+@BOTH
+def test_ignore_index_can_be_an_id(dtype):
+    h, w, t = make(120, 64, 50, dtype, seed=7)
+    check(h, w, t, ignore_index=int(t[5]))
+
+
+@BOTH
+@pytest.mark.parametrize("size", [1e-6, 40.0, 3000.0])
+def test_logits_of_every_size(size, dtype):
+    h, w, t = make(60, 128, 700, dtype, seed=9, scale=size)
+    h = torch.randn(60, 128, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    check(h, w, t)
+
+
+@BOTH
+def test_rows_of_very_different_sizes(dtype):
+    """Hidden rows, head rows and upstream gradients over several decades."""
+    h, w, t = make(130, 128, 600, dtype, seed=10)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = (w.float() * torch.pow(10.0, -3 * torch.rand(600, 1, generator=g, device="cuda"))).to(dtype)
+    h = (h.float() * torch.pow(10.0, 2 - 4 * torch.rand(130, 1, generator=g, device="cuda"))).to(dtype)
+    h[5] = 0
+    w[17] = 0
+    check(h, w, t)
+
+
+@BOTH
+def test_shapes_and_strides(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(6 * 33, 64, 500, dtype, seed=11)
+    plain = linear_cross_entropy(h, w, t, reduction="none")
+    wide = torch.full((6 * 33, 80), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 8:72] = h
+    assert torch.equal(linear_cross_entropy(wide[:, 8:72], w, t, reduction="none"), plain)          # a row stride
+    odd = torch.zeros(6 * 33 * 64 + 1, dtype=dtype, device="cuda")[1:].view(-1, 64).copy_(h)         # odd address
+    assert torch.equal(linear_cross_entropy(odd, w, t, reduction="none"), plain)
+    turned = h.t().contiguous().t()                                                                  # inner stride
+    assert torch.equal(linear_cross_entropy(turned, w, t, reduction="none"), plain)
+    cube, ids = h.view(6, 33, 64), t.view(6, 33)
+    shifted = linear_cross_entropy(cube[:, :-1], w, ids[:, 1:], reduction="none")
+    assert shifted.shape == (6, 32)
+    same = linear_cross_entropy(cube[:, :-1].reshape(-1, 64), w, ids[:, 1:].reshape(-1), reduction="none")
+    assert torch.equal(shifted.reshape(-1), same)
+    one = linear_cross_entropy(h[3], w, t[3], reduction="none")                                      # a single token
+    assert one.shape == () and abs(float(one - plain[3])) <= 1e-5 * float(plain[3])
+    repeated = h[:1].expand(5, 64)
+    assert torch.equal(linear_cross_entropy(repeated, w, t[:1].expand(5), reduction="none"), plain[:1].expand(5))
+
+
+@BOTH
+def test_a_broadcast_row_collects_every_gradient(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(20, 64, 300, dtype, seed=12)
+    row = h[:1].clone().requires_grad_(True)
+    (collected,) = torch.autograd.grad(linear_cross_entropy(row.expand(20, 64), w, t, reduction="sum"), row)
+    rows = h[:1].repeat(20, 1).requires_grad_(True)
+    (each,) = torch.autograd.grad(linear_cross_entropy(rows, w, t, reduction="sum"), rows)
+    assert torch.equal(collected, each.sum(0, keepdim=True))
+
+
+@BOTH
+def test_one_gradient_alone(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(77, 64, 400, dtype, seed=13)
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    both = torch.autograd.grad(linear_cross_entropy(hg, wg, t), (hg, wg))
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(hg, w, t), hg)[0], both[0])
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(h, wg, t), wg)[0], both[1])
+
+
+@BOTH
+def test_same_bits_on_every_call(dtype):
+    h, w, t = make(600, 256, 9000, dtype, seed=14, ignored=0.1)
+    first = check(h, w, t)
+    for _ in range(2):
+        for a, b in zip(first, check(h, w, t)):
+            assert torch.equal(a, b)
+
+
+def test_gradients_against_differences():
+    """A directional derivative of the summed loss in float32 by central differences: the loss is within its own bound
+    at both ends (divided by the step), and the third derivative of a log sum of exponentials along a direction that
+    moves the logits by at most R per unit is at most (2 R)^3 per row."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(24, 64, 200, torch.float32, seed=15)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    uh, uw = torch.randn(24, 64, generator=g, device="cuda"), torch.randn(200, 64, generator=g, device="cuda") / 8
+    hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dh, dw = torch.autograd.grad(linear_cross_entropy(hg, wg, t, reduction="sum"), (hg, wg))
+    for direction, grad, at in ((uh, dh, 0), (uw, dw, 1)):
+        step = 2.0 ** -7
+        ends, bound = [], 0.0
+        for sign in (1, -1):
+            hh, ww = (h + sign * step * direction, w) if at == 0 else (h, w + sign * step * direction)
+            ends.append(linear_cross_entropy(hh, ww, t, reduction="none").double().sum())
+            bound += float(reference(hh, ww, t, torch.ones(24, device="cuda"))[0][1].sum())
+        moved = (direction.double() @ w.double().T) if at == 0 else (h.double() @ direction.double().T)
+        curvature = float((2 * moved.abs().amax(1)).pow(3).sum()) * step ** 2 / 6
+        # perturbed inputs are rounded to float32 once: half a step of entries below 16
+        rounding = 16 * U * float(grad.double().abs().sum()) / step
+        slope = float((ends[0] - ends[1]) / (2 * step))
+        assert abs(slope - float((grad.double() * direction.double()).sum())) <= bound / (2 * step) + curvature + rounding
+
+
+@BOTH
+def test_another_stream_and_two_at_once(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    a, b = make(500, 128, 3000, dtype, seed=16), make(333, 64, 5000, dtype, seed=17, ignored=0.2)
+
+    def grads(case):
+        h, w = case[0].detach().requires_grad_(True), case[1].detach().requires_grad_(True)
+        loss = linear_cross_entropy(h, w, case[2])
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    expected = [grads(a), grads(b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        results = []
+        for stream, case in zip(streams, (a, b)):
+            with torch.cuda.stream(stream):
+                results.append(grads(case))
+        torch.cuda.synchronize()
+        for got, want in zip(results, expected):
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@BOTH
+@pytest.mark.parametrize("through_autograd", [False, True])
+def test_captured_and_replayed(through_autograd, dtype):
+    """A captured loss with its gradients, replayed on other inputs with another number of kept rows, two graphs in
+    turn. Outside autograd also while an eager graph of the same leaves lives."""
+    from hffn_b200.losses import linear_cross_entropy, linear_cross_entropy_gradients
+    h, w, t = make(400, 128, 2000, dtype, seed=18, ignored=0.1)
+    h, w = h.requires_grad_(True), w.requires_grad_(True)
+    eager = None if through_autograd else linear_cross_entropy(h, w, t)
+
+    def step(reduction):
+        if not through_autograd:
+            return linear_cross_entropy_gradients(h, w, t, reduction=reduction)
+        loss = linear_cross_entropy(h, w, t, reduction=reduction)
+        return (loss.detach(), *torch.autograd.grad(loss, (h, w)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step("mean"), step("sum")
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for reduction in ("mean", "sum"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(reduction))
+        graphs.append(graph)
+    for seed, ignored in ((19, 0.6), (20, 0.0), (21, 1.0)):
+        h2, w2, t2 = make(400, 128, 2000, dtype, seed=seed, ignored=ignored)
+        with torch.no_grad():
+            h.copy_(h2), w.copy_(w2), t.copy_(t2)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for reduction, got in zip(("mean", "sum"), outs):
+            assert all(torch.equal(x, y) for x, y in zip(got, step(reduction)))
+    assert eager is None or bool(torch.isfinite(eager))
+
+
+@BOTH
+def test_gradients_outside_autograd(dtype):
+    from hffn_b200.losses import linear_cross_entropy_gradients
+    h, w, t = make(96, 64, 700, dtype, seed=22, ignored=0.2)
+    c = torch.randn(96, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    for a, b in zip(check(h, w, t), linear_cross_entropy_gradients(h, w, t, c, reduction="none")):
+        assert torch.equal(a, b)
+    cube = linear_cross_entropy_gradients(h.view(4, 24, 64), w, t.view(4, 24))
+    assert cube[1].shape == (4, 24, 64) and cube[0].shape == ()
+    for a, b in zip(check(h, w, t, "mean"), cube):
+        assert torch.equal(a, b.view(a.shape))
+    with pytest.raises(ValueError):
+        linear_cross_entropy_gradients(h, w, t, c[:5], reduction="none")
+    with pytest.raises(ValueError):
+        linear_cross_entropy_gradients(h, w, t, c)
+
+
+def test_a_weight_changed_before_the_backward_is_noticed():
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(20, 64, 300, torch.float32)
+    h.requires_grad_(True)
+    loss = linear_cross_entropy(h, w, t)
+    w.add_(1.0)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+def test_refusals():
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(20, 64, 300, torch.float32)
+    for bad in (lambda: linear_cross_entropy(h, w, t, reduction="avg"),
+                lambda: linear_cross_entropy(h.half(), w.half(), t),
+                lambda: linear_cross_entropy(h.bfloat16(), w, t),
+                lambda: linear_cross_entropy(h, w, t.int()),
+                lambda: linear_cross_entropy(h, w, t.cpu()),
+                lambda: linear_cross_entropy(h, w, t[:19]),
+                lambda: linear_cross_entropy(h[:, :60], w[:, :60].contiguous(), t),
+                lambda: linear_cross_entropy(h[:, :56], w[:, :56], t),
+                lambda: linear_cross_entropy(h, torch.zeros(300 * 64 + 1, device="cuda")[1:].view(300, 64), t),
+                lambda: linear_cross_entropy(h, w[:0], t),
+                lambda: linear_cross_entropy(h[:0], w, t[:0])):
+        with pytest.raises(ValueError):
+            bad()
