@@ -111,6 +111,7 @@ SIGNATURES = {
     "hffn_linear_ce_backward_workspace": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
     "hffn_linear_ce_backward": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P, _P, _P, _P, _P, _I64, _I32, _I32,
                                                _P]),
+    "hffn_linear_ce_error": (ctypes.c_int, [ctypes.POINTER(_I32), ctypes.c_int]),
     "hffn_grad_norm_workspace": (_I64, [_I32]),
     "hffn_grad_norm": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, _P]),
     "hffn_clip_grad_norm": (ctypes.c_int, [_I32, _P, _P, _P, _P, _P, ctypes.c_float, _P, _P, _P]),

@@ -8,52 +8,123 @@
 // Only kept rows exist for the products: rows whose target is ignored (or out of range) are left out when the hidden
 // states are gathered, so they cost nothing and whatever they hold (infinities, NaN) reaches no sum. How many are
 // kept is known on the device alone; every kernel reads it there, so a call can be captured and replayed.
+//
+// The products (2 n vocab d operations each: the logits twice, dh, dw) bound everything from a few hundred tokens on;
+// below that the head's bytes do. All run in one persistent tcgen05 kernel shape on pairs of SMs (cta_group::2): a
+// tile of 256 x 256 accumulators, 128 rows in each SM's TMEM, each SM loading its own 128 rows of A and half of B, so
+// that an SM takes 32 KB from L2 per 64 values of K for 256 x 256 x 64 products of the pair. Two accumulator buffers let
+// the epilogue of one tile run under the products of the next.
+//
+// Types. bfloat16: products of the inputs as they are; g is held in bfloat16 (a rounding of 2^-9 on average per entry, of
+// the size of the gradients' own storage rounding), c_t included. float32: three fp16 products per product, of
+// operands held as two fp16 parts (hi = rn(x 2^e), lo = rn(x 2^e - hi); hi hi + hi lo + lo hi, the rest is below 2^-22),
+// 2^e one power of two per operand that brings its largest finite entry to [2^14, 2^15): entries down to 2^-17 of the
+// largest keep 22 bits, smaller ones are held to 2^-39 of it. One scale per operand, not per row, because each of h, w
+// and g is summed over its rows in one of the products. g holds 2^14 (p - [v = target]), c_t is applied in float32
+// afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). Sums: the
+// tensor core's float32 accumulation truncates, so float32 results are summed in registers from accumulators of kChunk
+// values of K each.
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
-#include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace hffn {
 namespace ce {
 
-constexpr int kRowTile = 256;                        // kept rows are padded to whole tiles (of zeros)
+using namespace tc;
+
+constexpr int kTile = 256;                           // rows and columns of a pair's tile
+constexpr int kBlockK = 64;                          // values of K in a stage: 128 bytes, the swizzle's row
+constexpr int kChunk = 4;                            // stages of K per accumulator (float32)
+constexpr int kThreads = 320;                        // warp 0: loads, warp 1: products, warps 2 to 9: epilogue
+constexpr int kEpilogueWarps = 8;
+constexpr int kGroupRows = 32;                       // row tiles of logits that share their pass over the vocabulary
+constexpr int kOperandBytes = 128 * kBlockK * 2;     // one SM's share of one operand part in a stage
+constexpr int kSmem = 6 * 2 * kOperandBytes + 1024 + 256;
 constexpr int64_t kPieceBytes = int64_t(256) << 20;  // of g: the piece of the vocabulary the backward holds at a time
 constexpr int kPieceMin = 4096;
+constexpr int kMaxDevices = 64;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kErrLoad = 401, kErrProduct = 402, kErrEpilogue = 403;
+
+__device__ int g_error;   // first error code of a wait that ran out (0: none)
 
 __host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // What the forward leaves for the backward, in one buffer.
 struct State {
   int32_t* kept;       // [1] rows kept
+  uint32_t* largest;   // [2] float32: bits of the largest finite |entry| of the kept rows and of the head
   int32_t* row_of;     // [n] the input row of each kept row
-  int32_t* place_of;   // [n] the kept row of each input row; -1: ignored, -2: target out of range
+  int32_t* place_of;   // [n] the kept row of each input row; -1: left out
   int32_t* target;     // [n]
   float* lse;          // [n]
-  void* hidden;        // [n_pad, d] the kept rows
+  void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts)
+  void* head[2];       // [vocab, d] float32: the head's fp16 parts
   int64_t bytes;
 };
 
-static State state_at(void* base, int dtype, int64_t n, int d) {
-  uint8_t* p = static_cast<uint8_t*>(base);
+struct Carve {
+  uint8_t* base;
   int64_t at = 0;
-  auto take = [&](int64_t bytes) {
-    uint8_t* q = p + at;
-    at += round_up(bytes, 256);
-    return q;
-  };
-  State s;
-  const int64_t n_pad = round_up(n, kRowTile);
-  s.kept = reinterpret_cast<int32_t*>(take(4));
-  s.row_of = reinterpret_cast<int32_t*>(take(4 * n_pad));
-  s.place_of = reinterpret_cast<int32_t*>(take(4 * n_pad));
-  s.target = reinterpret_cast<int32_t*>(take(4 * n_pad));
-  s.lse = reinterpret_cast<float*>(take(4 * n_pad));
-  s.hidden = take(n_pad * d * (dtype == HFFN_F32 ? 4 : 2));
-  s.bytes = at;
+  template <typename T>
+  T* take(int64_t count) {
+    T* p = reinterpret_cast<T*>(base + at);
+    at += round_up(count * (int64_t)sizeof(T), 256);
+    return p;
+  }
+};
+
+static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
+  Carve c{static_cast<uint8_t*>(base)};
+  const int64_t n_pad = round_up(n, kTile);
+  State s = {};
+  s.kept = c.take<int32_t>(4);
+  s.largest = reinterpret_cast<uint32_t*>(s.kept + 1);
+  s.row_of = c.take<int32_t>(n_pad);
+  s.place_of = c.take<int32_t>(n_pad);
+  s.target = c.take<int32_t>(n_pad);
+  s.lse = c.take<float>(n_pad);
+  for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
+  if (dtype == HFFN_F32)
+    for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
+  s.bytes = c.at;
   return s;
+}
+
+// ---- scales of the fp16 parts -------------------------------------------------------------------------------------
+// The exponent e of an operand's scale 2^e from the bits of its largest finite magnitude.
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  if (bits == 0) return 0;
+  return min(14 - ((int)(bits >> 23) - 127), 110);
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return ldexpf(1.f, e); }
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t bits = __float_as_uint(x) & 0x7fffffffu;
+  return bits < 0x7f800000u ? bits : 0u;
+}
+
+__device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
+  hi = __float2half_rn(x);
+  lo = __float2half_rn(x - __half2float(hi));
+}
+
+// Eight values as fp16 parts, 16 bytes each.
+__device__ __forceinline__ void store_parts(const float (&x)[8], __half* hi, __half* lo) {
+  __align__(16) __half h[8], l[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) split(x[j], h[j], l[j]);
+  *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(h);
+  *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(l);
 }
 
 // ---- which rows are kept ------------------------------------------------------------------------------------------
 constexpr int kGatherThreads = 256;
+constexpr int kGatherWarps = kGatherThreads / 32;
 
 __device__ __forceinline__ bool is_kept(int64_t target, int64_t ignore, int vocab) {
   return target != ignore && target >= 0 && target < vocab;
@@ -67,167 +138,712 @@ __device__ __forceinline__ int block_count(int mine, int* shared) {
   __syncthreads();
   int total = 0;
 #pragma unroll
-  for (int w = 0; w < kGatherThreads / 32; ++w) total += shared[w];
+  for (int w = 0; w < kGatherWarps; ++w) total += shared[w];
   return total;
 }
 
-// A block owns `span` consecutive input rows: it counts the kept rows before them (from the targets alone, so that no
-// block waits for another), places its own and copies them. The last block pads the kept rows to a whole tile of zeros.
+__device__ __forceinline__ void raise_largest(uint32_t* largest, uint32_t bits) {
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  if ((threadIdx.x & 31) == 0 && bits != 0) atomicMax(largest, bits);
+}
+
+// Blocks [0, gather): a block owns `span` consecutive input rows. It counts the kept rows before them (from the targets
+// alone, so that no block waits for another), places its own, and copies them (bfloat16) or raises the largest
+// magnitude by theirs (float32; a second kernel stores the parts). The last block zeroes the kept rows up to a whole
+// stage of K of the dw product. The other blocks (float32) raise the largest magnitude of the head.
 template <typename T>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden, int64_t stride, const int64_t* targets,
-                                                                int64_t ignore, int n, int d, int vocab, int span,
-                                                                State s) {
-  __shared__ int shared[kGatherThreads / 32];
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden, int64_t stride, const T* head,
+                                                                const int64_t* targets, int64_t ignore, int n, int d,
+                                                                int vocab, int span, int gather, bool aligned,
+                                                                float* losses, State s) {
+  constexpr bool kF32 = sizeof(T) == 4;
+  __shared__ int shared[kGatherWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (kF32 && blockIdx.x >= gather) {
+    const float4* from = reinterpret_cast<const float4*>(head);
+    const int64_t count = (int64_t)vocab * d / 4, step = (int64_t)(gridDim.x - gather) * kGatherThreads;
+    uint32_t bits = 0;
+#pragma unroll 4
+    for (int64_t i = (int64_t)(blockIdx.x - gather) * kGatherThreads + threadIdx.x; i < count; i += step) {
+      const float4 x = from[i];
+      bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
+    }
+    raise_largest(s.largest + 1, bits);
+    return;
+  }
   const int first = blockIdx.x * span, last = min(n, first + span);
   int mine = 0;
   for (int t = threadIdx.x; t < first; t += kGatherThreads) mine += is_kept(targets[t], ignore, vocab);
   int place = block_count(mine, shared);
-  T* out = static_cast<T*>(s.hidden);
-  for (int base = first; base < last; base += 32) {      // every warp walks all rows and copies every eighth
+  T* out = static_cast<T*>(s.hidden[0]);
+  uint32_t bits = 0;
+  for (int base = first; base < last; base += 32) {      // every warp walks all rows and takes every eighth kept one
     const int t = base + lane;
     const int64_t target = t < last ? targets[t] : ignore;
     const bool keep = t < last && is_kept(target, ignore, vocab);
     const unsigned mask = __ballot_sync(0xffffffffu, keep);
-    const int at = place + __popc(mask & ((1u << lane) - 1u));
     if (warp == 0 && t < last) {
-      s.place_of[t] = keep ? at : (target == ignore ? -1 : -2);
+      const int at = place + __popc(mask & ((1u << lane) - 1u));
+      s.place_of[t] = keep ? at : -1;
       if (keep) {
         s.row_of[at] = t;
         s.target[at] = (int)target;
+      } else {
+        losses[t] = target == ignore ? 0.f : NAN;
       }
     }
-    int k = 0;
-    for (unsigned left = mask; left; left &= left - 1, ++k) {
-      if (((place + k) & (kGatherThreads / 32 - 1)) != warp) continue;
+    int at = place;
+    for (unsigned left = mask; left; left &= left - 1, ++at) {
+      if ((at & (kGatherWarps - 1)) != warp) continue;
       const T* from = hidden + (int64_t)(base + __ffs(left) - 1) * stride;
-      T* to = out + (int64_t)(place + k) * d;
-      for (int i = lane; i < d; i += 32) to[i] = from[i];
+      if constexpr (kF32) {
+        for (int i = lane; i < d; i += 32) bits = max(bits, finite_bits(from[i]));
+      } else {
+        T* to = out + (int64_t)at * d;
+        if (aligned)
+          for (int i = lane; i < d / 8; i += 32)
+            reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
+        else
+          for (int i = lane; i < d; i += 32) to[i] = from[i];
+      }
     }
     place += __popc(mask);
   }
+  if (kF32) raise_largest(s.largest, bits);
   if (last == n) {
     if (threadIdx.x == 0) *s.kept = place;
-    const int64_t end = round_up(place, kRowTile) * d;
-    for (int64_t i = (int64_t)place * d + threadIdx.x; i < end; i += kGatherThreads) out[i] = from_f<T>(0.f);
+    const int64_t end = round_up(place, kBlockK) * d / 8;
+    for (int part = 0; part < (kF32 ? 2 : 1); ++part)
+      for (int64_t i = (int64_t)place * d / 8 + threadIdx.x; i < end; i += kGatherThreads)
+        static_cast<uint4*>(s.hidden[part])[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
+// float32: the fp16 parts of the head and of the kept rows, one warp a row.
+__global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t stride, bool aligned, const float* head,
+                                                    int d, int vocab, State s) {
+  const int lane = threadIdx.x & 31;
+  int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool of_head = row < vocab;
+  if (!of_head) row -= vocab;
+  if (!of_head && row >= *s.kept) return;
+  const float scale = power_of_two(scale_exponent(s.largest[of_head]));
+  const float* from = of_head ? head + (int64_t)row * d : hidden + (int64_t)s.row_of[row] * stride;
+  __half* hi = static_cast<__half*>(of_head ? s.head[0] : s.hidden[0]) + (int64_t)row * d;
+  __half* lo = static_cast<__half*>(of_head ? s.head[1] : s.hidden[1]) + (int64_t)row * d;
+  for (int i = 8 * lane; i < d; i += 256) {
+    float x[8];
+    if (of_head || aligned) {
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from + i);
+      *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(from + i + 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = from[i + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= scale;
+    store_parts(x, hi + i, lo + i);
+  }
+}
+
+// float32, a gradient of its own for each token: rows c_t h_t of the kept rows, first their largest magnitude, then
+// their fp16 parts (padded with zeros to a whole stage of K).
+template <bool kStore>
+__global__ void __launch_bounds__(256) scaled_rows_kernel(State s, const float* upstream, uint32_t* largest, __half* hi,
+                                                          __half* lo, int d) {
+  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), kept = *s.kept;
+  if (row >= (kStore ? (int)round_up(kept, kBlockK) : kept)) return;
+  const float inverse = power_of_two(-scale_exponent(s.largest[0]));
+  const float c = row < kept ? upstream[row] : 0.f;
+  const float scale = kStore ? power_of_two(scale_exponent(*largest)) : 1.f;
+  const __half* from_hi = static_cast<const __half*>(s.hidden[0]) + (int64_t)row * d;
+  const __half* from_lo = static_cast<const __half*>(s.hidden[1]) + (int64_t)row * d;
+  uint32_t bits = 0;
+  for (int i = 8 * lane; i < d; i += 256) {
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = row < kept ? c * ((__half2float(from_hi[i + j]) + __half2float(from_lo[i + j])) * inverse) : 0.f;
+      bits = max(bits, finite_bits(x[j]));
+      x[j] *= scale;
+    }
+    if (kStore) store_parts(x, hi + (int64_t)row * d + i, lo + (int64_t)row * d + i);
+  }
+  if (!kStore) raise_largest(largest, bits);
+}
+
 // ---- products -----------------------------------------------------------------------------------------------------
-// C[m, n] = sum_k A[m, k] B[n, k], either operand with any strides, 64 x 64 tiles, 4 x 4 values a thread.
-enum { kStats = 0, kGrad = 1, kGradHidden = 2, kGradWeight = 3 };
+// kStats: logits reduced to statistics. kGrad: logits turned into g. kGradients: dh and dw of one piece from g.
+enum Epilogue { kStats = 0, kGrad = 1, kGradients = 2 };
+
+// One product C[m, n] = sum_k A[m, k] B[n, k]. An operand is K-major (its rows hold consecutive k) or MN-major (its rows
+// hold consecutive m or n); kept: which of the three extents counts kept rows and is read on the device.
+struct Job {
+  int m, n, k;
+  int kept;                // 0: m, 2: k
+  int splits;              // parts of K, each a result of its own
+  int a_mn, b_mn;
+  int b_row;               // first row of B's tensor map that belongs to the product
+};
+
+struct Maps {
+  CUtensorMap a[2][2], b[2][2];   // [job][part]
+};
 
 struct Args {
   State s;
-  int v0;                  // first vocabulary row of the piece
-  int width;               // rows of the piece
-  float2* stats;           // [row tiles of the vocabulary][n_pad] maximum and sum of exponentials
-  float* picked;           // [n] the target's logit
-  const float* upstream;   // [n] c_t by kept row
-  float* g;                // [n_pad, width]
-  float* dh;               // [n_pad, d]
-  void* dw;                // [vocab, d]
-  int add;
+  Job job[2];
+  int jobs;
+  int d, vocab;
+  int v0, width;           // the piece of the vocabulary
+  int64_t n_pad;
+  float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials
+  float* picked;           // kStats: [n_pad] the target's logit
+  const float* upstream;   // [n_pad] c_t by kept row
+  void* g[2];              // kGrad: [n_pad, g_ld]
+  int64_t g_ld;
+  float* slots;            // kGradients: dh [splits][n_pad, d]
+  int add;                 // kGradients: dh adds to the slots (a later piece)
+  void* dw;                // kGradients: [vocab, d]
+  const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
+  const float* dw_factor;            // float32: one c for all rows, or NULL
 };
 
-constexpr int kTile = 64, kStep = 16;
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
 
-template <typename A, typename B, typename T, int EPI>
-__global__ void __launch_bounds__(256) product_kernel(const A* a, int64_t am, int64_t ak, const B* b, int64_t bn,
-                                                      int64_t bk, int M, int N, int K, int kept_dim, Args e, int d) {
-  const int kept = *e.s.kept;
-  if (kept_dim == 0) M = kept;       // the dimension that counts tokens
-  else K = kept;
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  if (m0 >= M) return;
-  __shared__ float as[kStep][kTile + 1], bs[kStep][kTile + 1];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += kStep) {
-    for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-      const int r = i / kStep, k = i % kStep;
-      as[k][r] = m0 + r < M && k0 + k < K ? to_f<A>(a[(m0 + r) * am + (k0 + k) * ak]) : 0.f;
-      bs[k][r] = n0 + r < N && k0 + k < K ? to_f<B>(b[(n0 + r) * bn + (k0 + k) * bk]) : 0.f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kStep; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty * 4 + i] * bs[k][tx * 4 + j];
-    __syncthreads();
+// The address of the first SM's copy of a shared-memory location, for accesses from either SM of the pair.
+__device__ __forceinline__ uint32_t at_leader(const void* p) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+  return a;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A tile load into this SM's shared memory, counted on the leader's barrier.
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint32_t leader_bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(leader_bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// Matrix descriptors over TMA's 128-byte swizzle. K-major: rows of 64 k (128 bytes), groups of 8 rows 1024 bytes apart.
+// MN-major: blocks of 64 m (128 bytes) x 64 k, 8192 bytes apart; within a block groups of 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn) {
+  const uint64_t leading = mn ? (8192 >> 4) : 1;
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (leading << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+
+__device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "r"(add));
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The extents of a launch's products, with the number of kept rows filled in.
+struct Extent {
+  int m_tiles, n_tiles, blocks, tiles;   // blocks of K
+};
+
+__device__ __forceinline__ Extent extent_of(const Job& j, int kept) {
+  Extent x;
+  x.m_tiles = ((j.kept == 0 ? kept : j.m) + kTile - 1) / kTile;
+  x.n_tiles = (j.n + kTile - 1) / kTile;
+  x.blocks = ((j.kept == 2 ? kept : j.k) + kBlockK - 1) / kBlockK;
+  x.tiles = x.m_tiles * x.n_tiles * j.splits;
+  return x;
+}
+
+struct Tile {
+  int job, m, n, split, first, last;     // blocks [first, last) of K
+};
+
+// Logits: all row tiles of a group before the next column tile, so that a tile of the head is read from HBM once per
+// group while the group's hidden states stay in L2. Gradients: the column tiles of a row tile together (they share A,
+// the long operand).
+template <int EPI>
+__device__ __forceinline__ Tile tile_of(int index, const Extent (&x)[2], const Args& e) {
+  Tile t;
+  t.job = EPI == kGradients && index >= x[0].tiles ? 1 : 0;
+  if (t.job) index -= x[0].tiles;
+  const Extent& q = t.job ? x[1] : x[0];
+  if constexpr (EPI == kGradients) {
+    t.n = index % q.n_tiles;
+    index /= q.n_tiles;
+    t.m = index % q.m_tiles;
+    t.split = index / q.m_tiles;
+    const int splits = e.job[t.job].splits;
+    t.first = (int)((int64_t)q.blocks * t.split / splits);
+    t.last = (int)((int64_t)q.blocks * (t.split + 1) / splits);
+  } else {
+    const int group = index / (kGroupRows * q.n_tiles), rest = index - group * kGroupRows * q.n_tiles;
+    const int rows = min(kGroupRows, q.m_tiles - group * kGroupRows);
+    t.n = rest / rows;
+    t.m = group * kGroupRows + rest % rows;
+    t.split = 0;
+    t.first = 0;
+    t.last = q.blocks;
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty * 4 + i;
-    if constexpr (EPI == kStats) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n0 + tx * 4 + j < N) top = fmaxf(top, acc[i][j]);
-#pragma unroll
-      for (int s = 8; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int v = n0 + tx * 4 + j;
-        if (v < N) sum += expf(acc[i][j] - top);
-        if (m < M && v < N && v == e.s.target[m]) e.picked[m] = acc[i][j];
+  return t;
+}
+
+// 32 columns of one row of the result, the accumulators `v` already scaled.
+template <int PARTS, int EPI>
+struct RowEpilogue {
+  const Args& e;
+  int row;                  // row of the product
+  bool live;                // it exists
+  int job, split;
+  // kStats
+  float top, sum;
+  int target;
+  // kGrad
+  float lse2, c;
+  // scale of the accumulators
+  float factor;
+
+  __device__ __forceinline__ RowEpilogue(const Args& args, const Tile& t, int row_in_tile, int kept) : e(args) {
+    row = t.m * kTile + row_in_tile;
+    job = t.job;
+    split = t.split;
+    factor = 1.f;
+    if constexpr (EPI == kGradients) {
+      live = row < (job == 0 ? kept : e.width);
+      if (PARTS == 2 && job == 1) {
+        factor = power_of_two(-14 - scale_exponent(*e.dw_rows_largest));
+        if (e.dw_factor != nullptr && kept > 0) factor *= *e.dw_factor;
       }
-#pragma unroll
-      for (int s = 8; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-      if (m < M && tx == 0) e.stats[(int64_t)blockIdx.x * gridDim.y * kTile + m] = make_float2(top, sum);
     } else {
-      if (m >= M) continue;
+      live = row < kept;
+      target = live ? e.s.target[row] : -1;
+      if (PARTS == 2) factor = power_of_two(-scale_exponent(e.s.largest[0]) - scale_exponent(e.s.largest[1]));
+      top = -INFINITY;
+      sum = 0.f;
+      if (EPI == kGrad) {
+        lse2 = live ? e.s.lse[row] * kLog2e : 0.f;
+        c = PARTS == 2 ? 16384.f : live ? e.upstream[row] : 0.f;
+      }
+    }
+  }
+
+  __device__ __forceinline__ void columns(float (&v)[32], int col) {
+    if constexpr (PARTS == 2) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = n0 + tx * 4 + j;
-        if (c >= N) continue;
-        if constexpr (EPI == kGrad) {
-          const float p = expf(acc[i][j] - e.s.lse[m]);
-          e.g[(int64_t)m * e.width + c] = e.upstream[m] * (p - (e.v0 + c == e.s.target[m] ? 1.f : 0.f));
-        } else if constexpr (EPI == kGradHidden) {
-          float* at = e.dh + (int64_t)m * d + c;
-          *at = acc[i][j] + (e.add ? *at : 0.f);
+      for (int j = 0; j < 32; ++j) v[j] *= factor;
+    }
+    if constexpr (EPI == kStats) {
+      if (col + 32 > e.vocab) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col + j >= e.vocab) v[j] = -INFINITY;
+      }
+      const int at = target - col;
+      if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (at == j) e.picked[row] = v[j];
+      }
+      float most = top;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) most = fmaxf(most, v[j]);
+      // a row of -inf so far has nothing to rescale; NaN logits reach the sum through their exponentials
+      const float base = most == -INFINITY ? 0.f : most * kLog2e;
+      float part[4] = {sum * exp2_fast(top * kLog2e - base), 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 32; ++j) part[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -base));
+      sum = (part[0] + part[1]) + (part[2] + part[3]);
+      top = most;
+    } else if constexpr (EPI == kGrad) {
+      const int at = target - e.v0 - col;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float p = exp2_fast(fmaf(v[j], kLog2e, -lse2));
+        v[j] = p;
+      }
+      if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (at == j) v[j] -= 1.f;
+      }
+      const int64_t to = (int64_t)row * e.g_ld + col;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = live ? c * v[8 * q + j] : 0.f;
+        if constexpr (PARTS == 2) {
+          store_parts(x, static_cast<__half*>(e.g[0]) + to + 8 * q, static_cast<__half*>(e.g[1]) + to + 8 * q);
         } else {
-          static_cast<T*>(e.dw)[(int64_t)(e.v0 + m) * d + c] = from_f<T>(acc[i][j]);
+          store8(static_cast<__nv_bfloat16*>(e.g[0]) + to + 8 * q, x);
+        }
+      }
+    } else {
+      if (!live) return;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (col + 8 * q >= e.d) break;       // d is a multiple of 8
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[8 * q + j];
+        if (job == 0) {
+          float4* to = reinterpret_cast<float4*>(e.slots + (split * e.n_pad + row) * e.d + col + 8 * q);
+          float4 a = make_float4(x[0], x[1], x[2], x[3]), b = make_float4(x[4], x[5], x[6], x[7]);
+          if (e.add) {
+            const float4 a0 = to[0], b0 = to[1];
+            a = make_float4(a.x + a0.x, a.y + a0.y, a.z + a0.z, a.w + a0.w);
+            b = make_float4(b.x + b0.x, b.y + b0.y, b.z + b0.z, b.w + b0.w);
+          }
+          to[0] = a;
+          to[1] = b;
+        } else {
+          const int64_t to = (int64_t)(e.v0 + row) * e.d + col + 8 * q;
+          if constexpr (PARTS == 2) {
+            float4* f = reinterpret_cast<float4*>(static_cast<float*>(e.dw) + to);
+            f[0] = make_float4(x[0], x[1], x[2], x[3]);
+            f[1] = make_float4(x[4], x[5], x[6], x[7]);
+          } else {
+            store8(static_cast<__nv_bfloat16*>(e.dw) + to, x);
+          }
         }
       }
     }
   }
+
+  __device__ __forceinline__ static void store8(__nv_bfloat16* to, const float (&x)[8]) {
+    __align__(16) __nv_bfloat162 h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(h);
+  }
+
+  __device__ __forceinline__ void finish(int column_part) {
+    if constexpr (EPI == kStats)
+      if (live) e.stats[column_part * e.n_pad + row] = make_float2(top, sum);
+  }
+};
+
+template <int PARTS>
+struct Stages {
+  static constexpr int kCount = 6 / PARTS;
+  static constexpr int kBytes = PARTS * 2 * kOperandBytes;   // of one SM
+};
+
+template <int PARTS, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e) {
+  constexpr int STAGES = Stages<PARTS>::kCount;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Stages<PARTS>::kBytes);   // used in the leader
+  uint64_t* empty = full + STAGES;
+  uint64_t* tfull = empty + STAGES;
+  uint64_t* tempty = tfull + 2;                                                          // used in the leader
+  uint64_t* done = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 2 * kEpilogueWarps);
+    }
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int kept = *e.s.kept;
+  const Extent extent[2] = {extent_of(e.job[0], kept), extent_of(e.job[1], kept)};
+  const int tiles = extent[0].tiles + (EPI == kGradients && e.jobs > 1 ? extent[1].tiles : 0);
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- loads ----------------
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int index = pair; index < tiles && ok; index += pairs) {
+        const Tile t = tile_of<EPI>(index, extent, e);
+        const Job& job = e.job[t.job];
+        const int m = t.m * kTile + (int)rank * 128, n = t.n * kTile + (int)rank * 128;
+        for (int kb = t.first; kb < t.last; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(&full[stage], 2 * Stages<PARTS>::kBytes);
+          const uint32_t bar = at_leader(&full[stage]);
+          uint8_t* dst = smem + stage * Stages<PARTS>::kBytes;
+          const int k = kb * kBlockK;
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            const CUtensorMap* a = &maps.a[t.job][part];
+            const CUtensorMap* b = &maps.b[t.job][part];
+            if (EPI == kGradients && job.a_mn) {
+              load_tile(dst, a, bar, m, k);
+              load_tile(dst + 8192, a, bar, m + 64, k);
+            } else {
+              load_tile(dst, a, bar, k, m);
+            }
+            dst += kOperandBytes;
+            if (EPI == kGradients && job.b_mn) {
+              load_tile(dst, b, bar, n, job.b_row + k);
+              load_tile(dst + 8192, b, bar, n + 64, job.b_row + k);
+            } else {
+              load_tile(dst, b, bar, k, job.b_row + n);
+            }
+            dst += kOperandBytes;
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        atomicCAS(&g_error, 0, kErrLoad);
+        *abort_flag = 1;
+        // the loads in flight land within microseconds; nothing waits on them any more, so this SM gives them time
+        const uint64_t start = global_ns();
+        while (global_ns() - start < 10000000ull) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // ---------------- products ----------------
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int index = pair; index < tiles && ok; index += pairs) {
+        const Tile t = tile_of<EPI>(index, extent, e);
+        const bool a_mn = EPI == kGradients && e.job[t.job].a_mn, b_mn = EPI == kGradients && e.job[t.job].b_mn;
+        constexpr uint32_t format = PARTS == 2 ? 0 : 1;   // fp16, bfloat16
+        const uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | ((uint32_t)a_mn << 15) |
+                               ((uint32_t)b_mn << 16) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+        const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;   // bytes of 16 k
+        const int chunk = PARTS == 2 ? kChunk : t.last - t.first;
+        for (int first = t.first; first < t.last && ok; first += chunk) {
+          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+          const uint32_t d_tmem = tmem_base + acc * kTile;
+          const int last = min(first + chunk, t.last);
+          for (int kb = first; kb < last; ++kb) {
+            if (!mbar_wait(&full[stage], phase, abort_flag, kWaitNs)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+            const uint32_t base = smem_u32(smem + stage * Stages<PARTS>::kBytes);
+#pragma unroll
+            for (int k = 0; k < kBlockK / 16; ++k) {
+              const uint64_t a = operand_desc(base + a_step * k, a_mn);
+              const uint64_t b = operand_desc(base + kOperandBytes + b_step * k, b_mn);
+              mma_pair(d_tmem, a, b, idesc, kb != first || k != 0);
+              if constexpr (PARTS == 2) {
+                const uint64_t a_lo = operand_desc(base + 2 * kOperandBytes + a_step * k, a_mn);
+                const uint64_t b_lo = operand_desc(base + 3 * kOperandBytes + b_step * k, b_mn);
+                mma_pair(d_tmem, a, b_lo, idesc, 1);
+                mma_pair(d_tmem, a_lo, b, idesc, 1);
+              }
+            }
+            commit_pair(&empty[stage]);
+            if (++stage == STAGES) {
+              stage = 0;
+              phase ^= 1;
+            }
+          }
+          if (!ok) break;
+          commit_pair(&tfull[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        atomicCAS(&g_error, 0, kErrProduct);
+        *abort_flag = 1;
+      }
+      // every product has been computed before the TMEM is freed
+      commit_pair(done);
+      const uint64_t start = global_ns();
+      while (!mbar_try_wait(done, 0) && global_ns() - start < kWaitNs) {
+      }
+    }
+  } else {
+    // ---------------- epilogue: a TMEM lane (row) per thread, two warps per lane quarter sharing the columns ----------
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
+    const int row_in_tile = (int)rank * 128 + quarter * 32 + lane;
+    const uint32_t release[2] = {at_leader(&tempty[0]), at_leader(&tempty[1])};
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int index = pair; index < tiles && ok; index += pairs) {
+      const Tile t = tile_of<EPI>(index, extent, e);
+      RowEpilogue<PARTS, EPI> out(e, t, row_in_tile, kept);
+      const int col = t.n * kTile + half * 128;
+      if constexpr (PARTS == 2) {
+        float total[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) total[j] = 0.f;
+        for (int first = t.first; first < t.last; first += kChunk) {
+          if (!mbar_wait(&tfull[acc], acc_phase, abort_flag, kWaitNs)) {
+            ok = false;
+            break;
+          }
+          fence_after();
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float v[32];
+            tmem_ld32(lane_base + acc * kTile + 32 * c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) total[32 * c + j] += v[j];
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(release[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = total[32 * c + j];
+          out.columns(v, col + 32 * c);
+        }
+      } else {
+        const bool any = t.first < t.last;
+        if (any && !mbar_wait(&tfull[acc], acc_phase, abort_flag, kWaitNs)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          float v[32];
+          if (any) {
+            tmem_ld32(lane_base + acc * kTile + 32 * c, v);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = 0.f;
+          }
+          out.columns(v, col + 32 * c);
+        }
+        if (any) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_at(release[acc]);
+          if (++acc == 2) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+      }
+      out.finish(2 * t.n + half);
+    }
+    if (!ok) {
+      if (lane == 0) atomicCAS(&g_error, 0, kErrEpilogue);
+      *abort_flag = 1;
+    }
+  }
+  __syncwarp();
+  fence_before();
+  __syncthreads();
+  cluster_sync();      // neither SM leaves while the other may still reach its memory or its barriers
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base));
+  }
 }
 
 // ---- per-row kernels ----------------------------------------------------------------------------------------------
-// lse and loss of each input row from the tiles' maxima and sums, one warp a row.
-__global__ void __launch_bounds__(256) losses_kernel(State s, const float2* stats, int64_t ld, int tiles,
-                                                     const float* picked, float* losses, int n) {
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= n) return;
-  const int at = s.place_of[t];
-  if (at < 0) {
-    if (lane == 0) losses[t] = at == -1 ? 0.f : NAN;
-    return;
-  }
+// lse and loss of the kept rows from the column parts' maxima and sums: 32 rows a block, its 32 warps sharing the parts.
+__device__ __forceinline__ void merge(float& top, float& sum, float top2, float sum2) {
+  const float most = fmaxf(top, top2);
+  if (most > -INFINITY) sum = sum * exp2f((top - most) * kLog2e) + sum2 * exp2f((top2 - most) * kLog2e);
+  else sum += sum2;
+  top = most;
+}
+
+__global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* stats, int64_t n_pad, int parts,
+                                                      const float* picked, float* losses) {
+  __shared__ float2 shared[32][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane, kept = *s.kept;
+  if (blockIdx.x * 32 >= kept) return;
   float top = -INFINITY, sum = 0.f;
-  for (int i = lane; i < tiles; i += 32) {
-    const float2 v = stats[i * ld + at];
-    const float m = fmaxf(top, v.x);
-    if (m > -INFINITY) sum = sum * expf(top - m) + v.y * expf(v.x - m);
-    else sum += v.y;
-    top = m;
+  if (row < kept) {
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 32) {
+      const float2 v = stats[i * n_pad + row];
+      merge(top, sum, v.x, v.y);
+    }
   }
+  shared[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  float2 v = shared[lane][warp];           // row `warp` of the block, one part a lane
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float top2 = __shfl_xor_sync(0xffffffffu, top, o), sum2 = __shfl_xor_sync(0xffffffffu, sum, o);
-    const float m = fmaxf(top, top2);
-    if (m > -INFINITY) sum = sum * expf(top - m) + sum2 * expf(top2 - m);
-    else sum += sum2;
-    top = m;
+    const float top2 = __shfl_xor_sync(0xffffffffu, v.x, o), sum2 = __shfl_xor_sync(0xffffffffu, v.y, o);
+    merge(v.x, v.y, top2, sum2);
   }
-  if (lane == 0) {
-    const float lse = top + logf(sum);
-    s.lse[at] = lse;
-    losses[t] = lse - picked[at];
+  const int mine = blockIdx.x * 32 + warp;
+  if (lane == 0 && mine < kept) {
+    const float lse = v.x + logf(v.y);
+    s.lse[mine] = lse;
+    losses[s.row_of[mine]] = lse - picked[mine];
   }
 }
 
@@ -255,30 +871,157 @@ __global__ void __launch_bounds__(256) upstream_kernel(State s, const float* gra
                  : reduction == HFFN_REDUCE_MEAN ? grad_loss[0] / (float)kept : grad_loss[0];
 }
 
-// dh of each input row: its kept row's, or zeros.
+// dh of each input row: the sum of its kept row's slots (in order), or zeros. One warp a row.
 template <typename T>
-__global__ void __launch_bounds__(256) scatter_kernel(State s, const float* dh, T* grad_hidden, int n, int d) {
+__global__ void __launch_bounds__(256) scatter_kernel(State s, const float* slots, int splits, int64_t n_pad,
+                                                      const float* upstream, T* grad_hidden, int n, int d) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t >= n) return;
   const int at = s.place_of[t];
-  for (int i = lane; i < d; i += 32) grad_hidden[(int64_t)t * d + i] = from_f<T>(at < 0 ? 0.f : dh[(int64_t)at * d + i]);
+  float factor = 1.f;
+  if (sizeof(T) == 4 && at >= 0) factor = upstream[at] * power_of_two(-14 - scale_exponent(s.largest[1]));
+  for (int i = 4 * lane; i < d; i += 128) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0)
+      for (int k = 0; k < splits; ++k) {
+        const float4 v = *reinterpret_cast<const float4*>(slots + (k * n_pad + at) * d + i);
+        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+      }
+    __align__(16) T out[4] = {from_f<T>(sum.x * factor), from_f<T>(sum.y * factor), from_f<T>(sum.z * factor),
+                              from_f<T>(sum.w * factor)};
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<float4*>(grad_hidden + (int64_t)t * d + i) = *reinterpret_cast<const float4*>(out);
+    else
+      *reinterpret_cast<uint2*>(grad_hidden + (int64_t)t * d + i) = *reinterpret_cast<const uint2*>(out);
+  }
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------
-static int piece_width(int64_t n, int vocab) {
-  const int64_t width = std::max<int64_t>(kPieceMin, kPieceBytes / 4 / round_up(n, kRowTile) / 256 * 256);
+static int parts_of(int dtype) { return dtype == HFFN_F32 ? 2 : 1; }
+
+// Columns of g held at a time: the vocabulary in equal pieces of whole tiles, each at most kPieceBytes but at least
+// kPieceMin columns (a shorter K would spend dh's time on adding its results to the last piece's).
+static int piece_width(int dtype, int64_t n, int vocab) {
+  const int64_t row = 2 * parts_of(dtype) * round_up(n, kTile);
+  const int64_t width = std::max<int64_t>(kPieceMin, kPieceBytes / row);
   const int64_t pieces = ceil_div(vocab, width);
-  return (int)std::min<int64_t>(vocab, round_up(ceil_div(vocab, pieces), 256));
+  return (int)round_up(ceil_div(vocab, pieces), kTile);
 }
 
-static int64_t forward_bytes(int64_t n, int vocab) {
-  const int64_t n_pad = round_up(n, kRowTile);
-  return round_up(8 * n_pad * ceil_div(vocab, kTile), 256) + 2 * round_up(4 * n_pad, 256);
+static int sm_pairs() {
+  static int pairs[kMaxDevices] = {};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) return 74;
+  if (pairs[device] == 0) {
+    int sms = 0;
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    pairs[device] = std::max(1, sms / 2);
+  }
+  return pairs[device];
 }
 
-static int64_t backward_bytes(int64_t n, int d, int vocab) {
-  const int64_t n_pad = round_up(n, kRowTile);
-  return round_up(4 * n_pad, 256) + round_up(4 * n_pad * piece_width(n, vocab), 256) + round_up(4 * n_pad * d, 256);
+// Parts of K of the dh product: as many as it takes to give every pair of SMs a tile, each part 1024 values at least.
+// From n alone, so that the result does not depend on the device.
+static int hidden_splits(int dtype, int64_t n, int d, int vocab) {
+  const int64_t tiles = ceil_div(n, kTile) * ceil_div(d, kTile);
+  const int64_t most = std::max<int64_t>(1, piece_width(dtype, n, vocab) / 1024);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, 74 / tiles));
+}
+
+static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t columns, int64_t ld,
+                    int box_rows) {
+  auto fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled unavailable");
+    return HFFN_ERR_CUDA;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows};
+  const cuuint32_t element[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == HFFN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed (%d) for a [%lld, %lld] operand", (int)r, (long long)rows,
+              (long long)columns);
+    return HFFN_ERR_CUDA;
+  }
+  return HFFN_OK;
+}
+
+template <int PARTS, int EPI>
+static int launch_products(const Maps& maps, const Args& e, int64_t most_tiles, cudaStream_t st) {
+  auto kernel = product_kernel<PARTS, EPI>;
+  static bool configured[kMaxDevices] = {};
+  int device = 0;
+  cudaGetDevice(&device);
+  if (device < 0 || device >= kMaxDevices || !configured[device]) {
+    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (r != cudaSuccess) {
+      set_error("linear_ce: %s", cudaGetErrorString(r));
+      return HFFN_ERR_CUDA;
+    }
+    if (device >= 0 && device < kMaxDevices) configured[device] = true;
+  }
+  const int pairs = (int)std::min<int64_t>(sm_pairs(), most_tiles);
+  kernel<<<2 * pairs, kThreads, kSmem, st>>>(maps, e);
+  return launch_status("linear_ce product");
+}
+
+// The logits' operands: rows of the kept hidden states and of the head, both K-major.
+static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_t n, int d, int vocab) {
+  const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
+  for (int part = 0; part < parts_of(dtype); ++part) {
+    HFFN_TRY(make_map(&maps.a[0][part], dtype, e.s.hidden[part], e.n_pad, d, d, 128));
+    HFFN_TRY(make_map(&maps.b[0][part], dtype, head[part], vocab, d, d, 128));
+  }
+  e.job[0] = {(int)n, e.width, d, 0, 1, 0, 0, e.v0};
+  e.job[1] = {};
+  e.jobs = 1;
+  return HFFN_OK;
+}
+
+struct ForwardWork {
+  float2* stats;
+  float *picked, *losses;
+  int64_t bytes;
+};
+
+static ForwardWork forward_work(void* base, int64_t n, int vocab) {
+  Carve c{static_cast<uint8_t*>(base)};
+  const int64_t n_pad = round_up(n, kTile);
+  ForwardWork w;
+  w.stats = c.take<float2>(2 * ceil_div(vocab, kTile) * n_pad);
+  w.picked = c.take<float>(n_pad);
+  w.losses = c.take<float>(n_pad);
+  w.bytes = c.at;
+  return w;
+}
+
+struct BackwardWork {
+  float* upstream;
+  void* g[2];
+  float* slots;
+  uint32_t* largest;      // float32, a gradient for each token: of c h
+  void* rows[2];          // and its fp16 parts
+  int64_t bytes;
+};
+
+static BackwardWork backward_work(void* base, int dtype, int64_t n, int d, int vocab) {
+  Carve c{static_cast<uint8_t*>(base)};
+  const int64_t n_pad = round_up(n, kTile);
+  BackwardWork w = {};
+  w.upstream = c.take<float>(n_pad);
+  for (int part = 0; part < parts_of(dtype); ++part) w.g[part] = c.take<uint16_t>(n_pad * piece_width(dtype, n, vocab));
+  w.slots = c.take<float>(hidden_splits(dtype, n, d, vocab) * n_pad * d);
+  if (dtype == HFFN_F32) {
+    w.largest = c.take<uint32_t>(1);
+    for (int part = 0; part < 2; ++part) w.rows[part] = c.take<uint16_t>(n_pad * d);
+  }
+  w.bytes = c.at;
+  return w;
 }
 
 static int check(int dtype, int64_t n, int32_t d, int32_t vocab) {
@@ -286,62 +1029,116 @@ static int check(int dtype, int64_t n, int32_t d, int32_t vocab) {
   HFFN_REQUIRE(n >= 1 && n <= (int64_t(1) << 24), "token count %lld out of range [1, 2^24]", (long long)n);
   HFFN_REQUIRE(d >= 8 && d % 8 == 0 && d <= 32768, "hidden size %d: a multiple of 8 up to 32768", d);
   HFFN_REQUIRE(vocab >= 1 && vocab <= (1 << 24), "vocabulary %d out of range [1, 2^24]", vocab);
+  HFFN_REQUIRE(ceil_div(n, kTile) * ceil_div(vocab, kTile) < (int64_t(1) << 30), "too many tokens times rows");
   return HFFN_OK;
 }
 
 template <typename T>
 static int forward(const void* hidden, int64_t stride, const void* weight, const int64_t* targets, int64_t ignore,
-                   int reduction, float* loss, const State& s, uint8_t* work, int n, int d, int vocab, cudaStream_t st) {
-  const int64_t n_pad = round_up(n, kRowTile);
-  const int tiles = (int)ceil_div(vocab, kTile);
+                   int reduction, float* loss, void* state, void* work, int n, int d, int vocab, cudaStream_t st) {
+  constexpr int PARTS = sizeof(T) / 2;
+  constexpr int dtype = PARTS == 2 ? HFFN_F32 : HFFN_BF16;
+  const ForwardWork w = forward_work(work, n, vocab);
   Args e = {};
-  e.s = s;
-  e.width = vocab;
-  e.stats = reinterpret_cast<float2*>(work);
-  e.picked = reinterpret_cast<float*>(work + round_up(8 * n_pad * tiles, 256));
-  float* losses = reduction == HFFN_REDUCE_NONE ? loss : e.picked + round_up(4 * n_pad, 256) / 4;
-  const int span = (int)std::max<int64_t>(16, ceil_div(n, 512));
-  gather_kernel<T><<<(unsigned)ceil_div(n, span), kGatherThreads, 0, st>>>(static_cast<const T*>(hidden), stride, targets,
-                                                                          ignore, n, d, vocab, span, s);
-  product_kernel<T, T, T, kStats><<<dim3(tiles, (unsigned)(n_pad / kTile)), 256, 0, st>>>(
-      static_cast<const T*>(s.hidden), d, 1, static_cast<const T*>(weight), d, 1, n, vocab, d, 0, e, d);
-  losses_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(s, e.stats, n_pad, tiles, e.picked, losses, n);
+  e.s = state_at(state, dtype, n, d, vocab);
+  e.d = d;
+  e.vocab = e.width = vocab;
+  e.n_pad = round_up(n, kTile);
+  e.stats = w.stats;
+  e.picked = w.picked;
+  float* losses = reduction == HFFN_REDUCE_NONE ? loss : w.losses;
+  const int span = (int)std::max<int64_t>(16, ceil_div(n, 512)), gather = (int)ceil_div(n, span);
+  const bool aligned = (reinterpret_cast<uintptr_t>(hidden) & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
+  if (PARTS == 2 && cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
+  const int measure = PARTS == 2 ? (int)std::min<int64_t>(148 * 8, ceil_div((int64_t)vocab * d, 4 * kGatherThreads)) : 0;
+  gather_kernel<T><<<gather + measure, kGatherThreads, 0, st>>>(static_cast<const T*>(hidden), stride,
+                                                                static_cast<const T*>(weight), targets, ignore, n, d,
+                                                                vocab, span, gather, aligned, losses, e.s);
+  if constexpr (PARTS == 2)
+    split_kernel<<<(unsigned)ceil_div((int64_t)vocab + n, 8), 256, 0, st>>>(
+        static_cast<const float*>(hidden), stride, aligned, static_cast<const float*>(weight), d, vocab, e.s);
+  Maps maps;
+  HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
+  HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), st)));
+  losses_kernel<<<(unsigned)ceil_div(n, 32), 1024, 0, st>>>(e.s, w.stats, e.n_pad, 2 * (int)ceil_div(vocab, kTile),
+                                                           w.picked, losses);
   if (reduction != HFFN_REDUCE_NONE)
-    reduce_kernel<<<1, 1024, 0, st>>>(s, losses, n, reduction == HFFN_REDUCE_MEAN, loss);
+    reduce_kernel<<<1, 1024, 0, st>>>(e.s, losses, n, reduction == HFFN_REDUCE_MEAN, loss);
   return launch_status("linear_ce_forward");
 }
 
 template <typename T>
 static int backward(const void* weight, int reduction, const float* grad_loss, void* grad_hidden, void* grad_weight,
-                    const State& s, uint8_t* work, int n, int d, int vocab, cudaStream_t st) {
-  const int64_t n_pad = round_up(n, kRowTile);
-  const int width = piece_width(n, vocab);
-  float* upstream = reinterpret_cast<float*>(work);
+                    void* state, void* work, int n, int d, int vocab, cudaStream_t st) {
+  constexpr int PARTS = sizeof(T) / 2;
+  constexpr int dtype = PARTS == 2 ? HFFN_F32 : HFFN_BF16;
+  const BackwardWork w = backward_work(work, dtype, n, d, vocab);
+  const int width = piece_width(dtype, n, vocab), splits = hidden_splits(dtype, n, d, vocab);
   Args e = {};
-  e.s = s;
-  e.upstream = upstream;
-  e.g = reinterpret_cast<float*>(work + round_up(4 * n_pad, 256));
-  e.dh = e.g + round_up(4 * n_pad * width, 256) / 4;
+  e.s = state_at(state, dtype, n, d, vocab);
+  e.d = d;
+  e.vocab = vocab;
+  e.n_pad = round_up(n, kTile);
+  e.upstream = w.upstream;
+  e.g[0] = w.g[0];
+  e.g[1] = w.g[1];
+  e.g_ld = width;
+  e.slots = w.slots;
   e.dw = grad_weight;
-  upstream_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(s, grad_loss, reduction, upstream);
-  const T *w = static_cast<const T*>(weight), *h = static_cast<const T*>(s.hidden);
+  upstream_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(e.s, grad_loss, reduction, w.upstream);
+  const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
+  if (PARTS == 2) {
+    e.dw_rows_largest = e.s.largest;
+    if (reduction != HFFN_REDUCE_NONE) {
+      e.dw_factor = w.upstream;
+    } else if (grad_weight != nullptr) {
+      e.dw_rows_largest = w.largest;
+      rows[0] = w.rows[0];
+      rows[1] = w.rows[1];
+      if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
+      __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
+      const unsigned blocks = (unsigned)(e.n_pad / 8);
+      scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, w.upstream, w.largest, hi, lo, d);
+      scaled_rows_kernel<true><<<blocks, 256, 0, st>>>(e.s, w.upstream, w.largest, hi, lo, d);
+    }
+  }
+  const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
+  const int64_t row_tiles = ceil_div(n, kTile), wide = ceil_div(d, kTile);
   for (int v0 = 0; v0 < vocab; v0 += width) {
     e.v0 = v0;
     e.width = std::min(width, vocab - v0);
     e.add = v0 > 0;
-    const T* piece = w + (int64_t)v0 * d;
-    const unsigned rows = (unsigned)(n_pad / kTile), cols = (unsigned)ceil_div(e.width, kTile);
-    const unsigned wide = (unsigned)ceil_div(d, kTile);
-    product_kernel<T, T, T, kGrad><<<dim3(cols, rows), 256, 0, st>>>(h, d, 1, piece, d, 1, n, e.width, d, 0, e, d);
-    if (grad_hidden != nullptr)
-      product_kernel<float, T, T, kGradHidden><<<dim3(wide, rows), 256, 0, st>>>(e.g, e.width, 1, piece, 1, d, n, d,
-                                                                                 e.width, 0, e, d);
-    if (grad_weight != nullptr)
-      product_kernel<float, T, T, kGradWeight><<<dim3(wide, cols), 256, 0, st>>>(e.g, 1, e.width, h, 1, d, e.width, d,
-                                                                                 n, 1, e, d);
+    const int64_t columns = ceil_div(e.width, kTile);
+    Maps maps;
+    HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
+    HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, st)));
+    e.jobs = 0;
+    int64_t tiles = 0;
+    if (grad_hidden != nullptr) {
+      const int j = e.jobs++;
+      for (int part = 0; part < PARTS; ++part) {
+        HFFN_TRY(make_map(&maps.a[j][part], dtype, w.g[part], e.n_pad, e.width, width, 128));
+        HFFN_TRY(make_map(&maps.b[j][part], dtype, head[part], vocab, d, d, kBlockK));
+      }
+      e.job[j] = {n, d, e.width, 0, splits, 0, 1, v0};
+      tiles += row_tiles * wide * splits;
+    }
+    if (grad_weight != nullptr) {
+      // job 1 is dw: without dh, job 0 is empty
+      if (e.jobs == 0) e.job[e.jobs++] = {};
+      for (int part = 0; part < PARTS; ++part) {
+        HFFN_TRY(make_map(&maps.a[1][part], dtype, w.g[part], e.n_pad, e.width, width, kBlockK));
+        HFFN_TRY(make_map(&maps.b[1][part], dtype, rows[part], e.n_pad, d, d, kBlockK));
+      }
+      e.job[1] = {e.width, d, n, 2, 1, 1, 1, 0};
+      e.jobs = 2;
+      tiles += columns * wide;
+    }
+    if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, st)));
   }
   if (grad_hidden != nullptr)
-    scatter_kernel<T><<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(s, e.dh, static_cast<T*>(grad_hidden), n, d);
+    scatter_kernel<T><<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(e.s, w.slots, splits, e.n_pad, w.upstream,
+                                                                static_cast<T*>(grad_hidden), n, d);
   return launch_status("linear_ce_backward");
 }
 
@@ -356,17 +1153,17 @@ extern "C" {
 
 int64_t hffn_linear_ce_state_bytes(int dtype, int64_t n, int32_t d, int32_t vocab) {
   if (ce::check(dtype, n, d, vocab) != HFFN_OK) return -1;
-  return ce::state_at(nullptr, dtype, n, d).bytes;
+  return ce::state_at(nullptr, dtype, n, d, vocab).bytes;
 }
 
 int64_t hffn_linear_ce_forward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab) {
   if (ce::check(dtype, n, d, vocab) != HFFN_OK) return -1;
-  return ce::forward_bytes(n, vocab);
+  return ce::forward_work(nullptr, n, vocab).bytes;
 }
 
 int64_t hffn_linear_ce_backward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab) {
   if (ce::check(dtype, n, d, vocab) != HFFN_OK) return -1;
-  return ce::backward_bytes(n, d, vocab);
+  return ce::backward_work(nullptr, dtype, n, d, vocab).bytes;
 }
 
 int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
@@ -380,10 +1177,9 @@ int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride,
   HFFN_REQUIRE(ce::aligned16(weight) && ce::aligned16(state) && ce::aligned16(work),
                "weight, state and work must be 16-byte aligned");
   HFFN_TRY(bind_stream_device(stream));
-  const ce::State s = ce::state_at(state, dtype, n, d);
   auto run = dtype == HFFN_F32 ? ce::forward<float> : ce::forward<__nv_bfloat16>;
-  return run(hidden, hidden_stride, weight, targets, ignore_index, reduction, loss, s, static_cast<uint8_t*>(work),
-             (int)n, d, vocab, static_cast<cudaStream_t>(stream));
+  return run(hidden, hidden_stride, weight, targets, ignore_index, reduction, loss, state, work, (int)n, d, vocab,
+             static_cast<cudaStream_t>(stream));
 }
 
 int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const float* grad_loss, void* grad_hidden,
@@ -397,10 +1193,23 @@ int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const 
                    ce::aligned16(grad_weight),
                "weight, gradients, state and work must be 16-byte aligned");
   HFFN_TRY(bind_stream_device(stream));
-  const ce::State s = ce::state_at(state, dtype, n, d);
   auto run = dtype == HFFN_F32 ? ce::backward<float> : ce::backward<__nv_bfloat16>;
-  return run(weight, reduction, grad_loss, grad_hidden, grad_weight, s, static_cast<uint8_t*>(work), (int)n, d, vocab,
+  return run(weight, reduction, grad_loss, grad_hidden, grad_weight, state, work, (int)n, d, vocab,
              static_cast<cudaStream_t>(stream));
+}
+
+int hffn_linear_ce_error(int32_t* value, int clear) {
+  HFFN_REQUIRE(value != nullptr, "null pointer argument");
+  cudaError_t e = cudaMemcpyFromSymbol(value, ce::g_error, sizeof(int32_t));
+  if (e == cudaSuccess && clear) {
+    const int32_t zero = 0;
+    e = cudaMemcpyToSymbol(ce::g_error, &zero, sizeof(int32_t));
+  }
+  if (e != cudaSuccess) {
+    set_error("hffn_linear_ce_error: %s", cudaGetErrorString(e));
+    return HFFN_ERR_CUDA;
+  }
+  return HFFN_OK;
 }
 
 }  // extern "C"

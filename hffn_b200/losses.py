@@ -128,3 +128,12 @@ def linear_cross_entropy_gradients(hidden: torch.Tensor, weight: torch.Tensor, t
     grad_loss = torch.ones_like(loss) if grad_loss is None else grad_loss.reshape(loss.shape)
     grad_hidden, grad_weight = _backward(weight, state, targets.numel(), reduction, grad_loss)
     return loss.view(shape), grad_hidden.view(hidden.shape), grad_weight
+
+
+def device_errors(device=None) -> int:
+    """The error flag of the loss's kernels on ``device`` (0: none; the code of a wait that ran out otherwise).
+    Synchronises."""
+    flag = native.ctypes.c_int32(0)
+    with torch.cuda.device(device):
+        native.check(native.lib.hffn_linear_ce_error(native.ctypes.byref(flag), 0), "hffn_linear_ce_error")
+    return int(flag.value)

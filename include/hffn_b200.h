@@ -384,6 +384,10 @@ int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const 
                             void* grad_weight, void* state, void* work, int64_t n, int32_t d, int32_t vocab,
                             void* stream);
 
+/* The error flag of those kernels on the current device: 0, or the code of the first bounded wait that ran out (401, 402,
+ * 403). Synchronous; clear != 0 resets it. */
+int hffn_linear_ce_error(int32_t* value, int clear);
+
 /* The 2-norm over every entry of `count` tensors (no counterpart in the reference): tensors[i] holds numel[i] entries of
  * dtypes[i] (the lists are host arrays, read before the call returns), summed in float64; *norm: float32 on the
  * device. work: hffn_grad_norm_workspace bytes, 8-byte aligned. */

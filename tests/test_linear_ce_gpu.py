@@ -112,6 +112,13 @@ def check(h, w, targets, reduction="none", seed=3, ignore_index=IGNORE):
     return loss.detach(), dh, dw
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    from hffn_b200.losses import device_errors
+    assert device_errors() == 0
+
+
 BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 SHAPES = [(1, 8, 1), (1, 64, 2), (2, 72, 7), (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
           (256, 512, 1000), (257, 1024, 2049), (700, 328, 4099), (1, 1024, 50304), (9, 2048, 5001), (1021, 768, 3001)]
