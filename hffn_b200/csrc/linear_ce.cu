@@ -276,13 +276,14 @@ __global__ void __launch_bounds__(256) scaled_rows_kernel(State s, const float* 
 // kStats: logits reduced to statistics. kGrad: logits turned into g. kGradients: dh and dw of one piece from g.
 enum Epilogue { kStats = 0, kGrad = 1, kGradients = 2 };
 
-// One product C[m, n] = sum_k A[m, k] B[n, k]. An operand is K-major (its rows hold consecutive k) or MN-major (its rows
-// hold consecutive m or n); kept: which of the three extents counts kept rows and is read on the device.
+// One product C[m, n] = sum_k A[m, k] B[n, k]; kept: which of the three extents counts kept rows and is read on the
+// device. An operand is K-major (its rows hold consecutive k) or MN-major (its rows hold consecutive m or n): the logits'
+// are both K-major, dh (job 0 of kGradients) has B MN-major (the head as it is), dw (job 1) both (g and the hidden
+// states as they are).
 struct Job {
   int m, n, k;
   int kept;                // 0: m, 2: k
   int splits;              // parts of K, each a result of its own
-  int a_mn, b_mn;
   int b_row;               // first row of B's tensor map that belongs to the product
 };
 
@@ -556,6 +557,117 @@ struct Stages {
   static constexpr int kBytes = PARTS * 2 * kOperandBytes;   // of one SM
 };
 
+// A position in a ring of `count` slots whose barriers' phases alternate.
+struct Ring {
+  int at = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int count) {
+    if (++at == count) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t elected;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+  return elected != 0;
+}
+
+// A bounded wait of a whole warp: every lane gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kWaitNs));
+}
+
+template <int EPI, int JOB>
+struct Major {
+  static constexpr bool kA = EPI == kGradients && JOB == 1, kB = EPI == kGradients;   // MN-major
+};
+
+// The loads of one tile's K. The whole warp runs the loop and one lane issues, with the tensor maps at addresses known
+// when compiled: from one lane alone, or with a map picked at run time, a stage's three or four loads took 550 cycles to
+// issue, longer than its products (dh 8192 x 2048 x 12800: 801 cycles a stage, 586 for the logits).
+template <int PARTS, int EPI, int JOB>
+__device__ __forceinline__ bool load_stages(const Maps& maps, const Args& e, const Tile& t, uint32_t rank, uint8_t* smem,
+                                            uint64_t* full, uint64_t* empty, Ring& ring, volatile int* abort_flag) {
+  using M = Major<EPI, JOB>;
+  const int m = t.m * kTile + (int)rank * 128, n = t.n * kTile + (int)rank * 128, b_row = e.job[JOB].b_row;
+  for (int kb = t.first; kb < t.last; ++kb) {
+    if (!warp_wait(&empty[ring.at], ring.phase ^ 1, abort_flag)) return false;
+    if (elect_one()) {
+      if (rank == 0) mbar_expect_tx(&full[ring.at], 2 * Stages<PARTS>::kBytes);
+      const uint32_t bar = at_leader(&full[ring.at]);
+      uint8_t* dst = smem + ring.at * Stages<PARTS>::kBytes;
+      const int k = kb * kBlockK;
+#pragma unroll
+      for (int part = 0; part < PARTS; ++part) {
+        if constexpr (M::kA) {
+          load_tile(dst, &maps.a[JOB][part], bar, m, k);
+          load_tile(dst + 8192, &maps.a[JOB][part], bar, m + 64, k);
+        } else {
+          load_tile(dst, &maps.a[JOB][part], bar, k, m);
+        }
+        dst += kOperandBytes;
+        if constexpr (M::kB) {
+          load_tile(dst, &maps.b[JOB][part], bar, n, b_row + k);
+          load_tile(dst + 8192, &maps.b[JOB][part], bar, n + 64, b_row + k);
+        } else {
+          load_tile(dst, &maps.b[JOB][part], bar, k, b_row + n);
+        }
+        dst += kOperandBytes;
+      }
+    }
+    __syncwarp();
+    ring.next(Stages<PARTS>::kCount);
+  }
+  return true;
+}
+
+// The products of one tile, kChunk stages per accumulator (float32) or all of them.
+template <int PARTS, int EPI, int JOB>
+__device__ __forceinline__ bool multiply_stages(const Tile& t, uint32_t tmem_base, uint8_t* smem, uint64_t* full,
+                                                uint64_t* empty, uint64_t* tfull, uint64_t* tempty, Ring& ring, Ring& acc,
+                                                volatile int* abort_flag) {
+  using M = Major<EPI, JOB>;
+  constexpr uint32_t format = PARTS == 2 ? 0 : 1;   // fp16, bfloat16
+  constexpr uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | ((uint32_t)M::kA << 15) |
+                             ((uint32_t)M::kB << 16) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+  constexpr uint32_t a_step = M::kA ? 2048 : 32, b_step = M::kB ? 2048 : 32;   // bytes of 16 k
+  const int chunk = PARTS == 2 ? kChunk : t.last - t.first;
+  for (int first = t.first; first < t.last; first += chunk) {
+    if (!warp_wait(&tempty[acc.at], acc.phase ^ 1, abort_flag)) return false;
+    fence_after();
+    const uint32_t d_tmem = tmem_base + acc.at * kTile;
+    const int last = min(first + chunk, t.last);
+    for (int kb = first; kb < last; ++kb) {
+      if (!warp_wait(&full[ring.at], ring.phase, abort_flag)) return false;
+      fence_after();
+      if (elect_one()) {
+        const uint32_t base = smem_u32(smem + ring.at * Stages<PARTS>::kBytes);
+#pragma unroll
+        for (int k = 0; k < kBlockK / 16; ++k) {
+          const uint64_t a = operand_desc(base + a_step * k, M::kA);
+          const uint64_t b = operand_desc(base + kOperandBytes + b_step * k, M::kB);
+          mma_pair(d_tmem, a, b, idesc, kb != first || k != 0);
+          if constexpr (PARTS == 2) {
+            const uint64_t a_lo = operand_desc(base + 2 * kOperandBytes + a_step * k, M::kA);
+            const uint64_t b_lo = operand_desc(base + 3 * kOperandBytes + b_step * k, M::kB);
+            mma_pair(d_tmem, a, b_lo, idesc, 1);
+            mma_pair(d_tmem, a_lo, b, idesc, 1);
+          }
+        }
+        commit_pair(&empty[ring.at]);
+        if (kb == last - 1) commit_pair(&tfull[acc.at]);
+      }
+      __syncwarp();
+      ring.next(Stages<PARTS>::kCount);
+    }
+    acc.next(2);
+  }
+  return true;
+}
+
 template <int PARTS, int EPI>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e) {
@@ -601,121 +713,49 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- loads ----------------
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int index = pair; index < tiles && ok; index += pairs) {
-        const Tile t = tile_of<EPI>(index, extent, e);
-        const Job& job = e.job[t.job];
-        const int m = t.m * kTile + (int)rank * 128, n = t.n * kTile + (int)rank * 128;
-        for (int kb = t.first; kb < t.last; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1, abort_flag, kWaitNs)) {
-            ok = false;
-            break;
-          }
-          if (rank == 0) mbar_expect_tx(&full[stage], 2 * Stages<PARTS>::kBytes);
-          const uint32_t bar = at_leader(&full[stage]);
-          uint8_t* dst = smem + stage * Stages<PARTS>::kBytes;
-          const int k = kb * kBlockK;
-#pragma unroll
-          for (int part = 0; part < PARTS; ++part) {
-            const CUtensorMap* a = &maps.a[t.job][part];
-            const CUtensorMap* b = &maps.b[t.job][part];
-            if (EPI == kGradients && job.a_mn) {
-              load_tile(dst, a, bar, m, k);
-              load_tile(dst + 8192, a, bar, m + 64, k);
-            } else {
-              load_tile(dst, a, bar, k, m);
-            }
-            dst += kOperandBytes;
-            if (EPI == kGradients && job.b_mn) {
-              load_tile(dst, b, bar, n, job.b_row + k);
-              load_tile(dst + 8192, b, bar, n + 64, job.b_row + k);
-            } else {
-              load_tile(dst, b, bar, k, job.b_row + n);
-            }
-            dst += kOperandBytes;
-          }
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
-        }
-      }
-      if (!ok) {
-        atomicCAS(&g_error, 0, kErrLoad);
-        *abort_flag = 1;
-        // the loads in flight land within microseconds; nothing waits on them any more, so this SM gives them time
-        const uint64_t start = global_ns();
-        while (global_ns() - start < 10000000ull) {
-        }
+    // ---------------- loads ----------------
+    Ring ring;
+    bool ok = true;
+    for (int index = pair; index < tiles && ok; index += pairs) {
+      const Tile t = tile_of<EPI>(index, extent, e);
+      if (EPI == kGradients && t.job == 1)
+        ok = load_stages<PARTS, EPI, 1>(maps, e, t, rank, smem, full, empty, ring, abort_flag);
+      else
+        ok = load_stages<PARTS, EPI, 0>(maps, e, t, rank, smem, full, empty, ring, abort_flag);
+    }
+    if (!ok && lane == 0) {
+      atomicCAS(&g_error, 0, kErrLoad);
+      *abort_flag = 1;
+      // the loads in flight land within microseconds; nothing waits on them any more, so this SM gives them time
+      const uint64_t start = global_ns();
+      while (global_ns() - start < 10000000ull) {
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---------------- products ----------------
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      Ring ring, acc;
       bool ok = true;
       for (int index = pair; index < tiles && ok; index += pairs) {
         const Tile t = tile_of<EPI>(index, extent, e);
-        const bool a_mn = EPI == kGradients && e.job[t.job].a_mn, b_mn = EPI == kGradients && e.job[t.job].b_mn;
-        constexpr uint32_t format = PARTS == 2 ? 0 : 1;   // fp16, bfloat16
-        const uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | ((uint32_t)a_mn << 15) |
-                               ((uint32_t)b_mn << 16) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
-        const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;   // bytes of 16 k
-        const int chunk = PARTS == 2 ? kChunk : t.last - t.first;
-        for (int first = t.first; first < t.last && ok; first += chunk) {
-          if (!mbar_wait(&tempty[acc], acc_phase ^ 1, abort_flag, kWaitNs)) {
-            ok = false;
-            break;
-          }
-          fence_after();
-          const uint32_t d_tmem = tmem_base + acc * kTile;
-          const int last = min(first + chunk, t.last);
-          for (int kb = first; kb < last; ++kb) {
-            if (!mbar_wait(&full[stage], phase, abort_flag, kWaitNs)) {
-              ok = false;
-              break;
-            }
-            fence_after();
-            const uint32_t base = smem_u32(smem + stage * Stages<PARTS>::kBytes);
-#pragma unroll
-            for (int k = 0; k < kBlockK / 16; ++k) {
-              const uint64_t a = operand_desc(base + a_step * k, a_mn);
-              const uint64_t b = operand_desc(base + kOperandBytes + b_step * k, b_mn);
-              mma_pair(d_tmem, a, b, idesc, kb != first || k != 0);
-              if constexpr (PARTS == 2) {
-                const uint64_t a_lo = operand_desc(base + 2 * kOperandBytes + a_step * k, a_mn);
-                const uint64_t b_lo = operand_desc(base + 3 * kOperandBytes + b_step * k, b_mn);
-                mma_pair(d_tmem, a, b_lo, idesc, 1);
-                mma_pair(d_tmem, a_lo, b, idesc, 1);
-              }
-            }
-            commit_pair(&empty[stage]);
-            if (++stage == STAGES) {
-              stage = 0;
-              phase ^= 1;
-            }
-          }
-          if (!ok) break;
-          commit_pair(&tfull[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
+        if (EPI == kGradients && t.job == 1)
+          ok = multiply_stages<PARTS, EPI, 1>(t, tmem_base, smem, full, empty, tfull, tempty, ring, acc, abort_flag);
+        else
+          ok = multiply_stages<PARTS, EPI, 0>(t, tmem_base, smem, full, empty, tfull, tempty, ring, acc, abort_flag);
+      }
+      if (lane == 0) {
+        if (!ok) {
+          atomicCAS(&g_error, 0, kErrProduct);
+          *abort_flag = 1;
         }
       }
-      if (!ok) {
-        atomicCAS(&g_error, 0, kErrProduct);
-        *abort_flag = 1;
-      }
-      // every product has been computed before the TMEM is freed
-      commit_pair(done);
-      const uint64_t start = global_ns();
-      while (!mbar_try_wait(done, 0) && global_ns() - start < kWaitNs) {
+      __syncwarp();
+      // every product has been computed before the TMEM is freed (tcgen05.commit tracks the elected lane's products)
+      if (elect_one()) {
+        commit_pair(done);
+        const uint64_t start = global_ns();
+        while (!mbar_try_wait(done, 0) && global_ns() - start < kWaitNs) {
+        }
       }
     }
   } else {
@@ -977,7 +1017,7 @@ static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_
     HFFN_TRY(make_map(&maps.a[0][part], dtype, e.s.hidden[part], e.n_pad, d, d, 128));
     HFFN_TRY(make_map(&maps.b[0][part], dtype, head[part], vocab, d, d, 128));
   }
-  e.job[0] = {(int)n, e.width, d, 0, 1, 0, 0, e.v0};
+  e.job[0] = {(int)n, e.width, d, 0, 1, e.v0};
   e.job[1] = {};
   e.jobs = 1;
   return HFFN_OK;
@@ -1120,7 +1160,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
         HFFN_TRY(make_map(&maps.a[j][part], dtype, w.g[part], e.n_pad, e.width, width, 128));
         HFFN_TRY(make_map(&maps.b[j][part], dtype, head[part], vocab, d, d, kBlockK));
       }
-      e.job[j] = {n, d, e.width, 0, splits, 0, 1, v0};
+      e.job[j] = {n, d, e.width, 0, splits, v0};
       tiles += row_tiles * wide * splits;
     }
     if (grad_weight != nullptr) {
@@ -1130,7 +1170,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
         HFFN_TRY(make_map(&maps.a[1][part], dtype, w.g[part], e.n_pad, e.width, width, kBlockK));
         HFFN_TRY(make_map(&maps.b[1][part], dtype, rows[part], e.n_pad, d, d, kBlockK));
       }
-      e.job[1] = {e.width, d, n, 2, 1, 1, 1, 0};
+      e.job[1] = {e.width, d, n, 2, 1, 0};
       e.jobs = 2;
       tiles += columns * wide;
     }
