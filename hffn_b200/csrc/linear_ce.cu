@@ -42,7 +42,9 @@ constexpr int kThreads = 320;                        // warp 0: loads, warp 1: p
 constexpr int kEpilogueWarps = 8;
 constexpr int kGroupRows = 32;                       // row tiles of logits that share their pass over the vocabulary
 constexpr int kOperandBytes = 128 * kBlockK * 2;     // one SM's share of one operand part in a stage
-constexpr int kSmem = 6 * 2 * kOperandBytes + 1024 + 256;
+constexpr int kStageBytes = 6 * 2 * kOperandBytes;     // all stages of one SM
+constexpr int kOutBytes = 4096;                      // an epilogue warp's 32 rows x 32 columns on their way out
+constexpr int kSmem = 1024 + kStageBytes + kEpilogueWarps * kOutBytes + 256;
 constexpr int64_t kPieceBytes = int64_t(256) << 20;  // of g: the piece of the vocabulary the backward holds at a time
 constexpr int kPieceMin = 4096;
 constexpr int kMaxDevices = 64;
@@ -289,6 +291,7 @@ struct Job {
 
 struct Maps {
   CUtensorMap a[2][2], b[2][2];   // [job][part]
+  CUtensorMap out[2];             // kGrad: g's parts; kGradients: dh's slots, dw
 };
 
 struct Args {
@@ -301,11 +304,7 @@ struct Args {
   float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials
   float* picked;           // kStats: [n_pad] the target's logit
   const float* upstream;   // [n_pad] c_t by kept row
-  void* g[2];              // kGrad: [n_pad, g_ld]
-  int64_t g_ld;
-  float* slots;            // kGradients: dh [splits][n_pad, d]
-  int add;                 // kGradients: dh adds to the slots (a later piece)
-  void* dw;                // kGradients: [vocab, d]
+  int add;                 // kGradients: dh adds to its slots (a later piece)
   const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
   const float* dw_factor;            // float32: one c for all rows, or NULL
 };
@@ -416,29 +415,80 @@ __device__ __forceinline__ Tile tile_of(int index, const Extent (&x)[2], const A
   return t;
 }
 
-// 32 columns of one row of the result, the accumulators `v` already scaled.
+// A warp's 32 x 32 block of a result on its way to global memory: rows of 64 or 128 bytes in the swizzle TMA reads, so
+// that a row's 16-byte pieces fall in different banks across rows, then one tile store. Stored by each thread for its
+// own row instead, every 16 bytes of a warp's store touch another line: 32 passes through the L1 per instruction, which
+// bounded g (d 1024, bfloat16: 906 us against 647 for the same logits without a store).
+struct BlockOut {
+  uint8_t* base;
+  int lane;
+
+  __device__ __forceinline__ void begin() const {      // the last block has been read out
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+  }
+  template <int ROW_BYTES>
+  __device__ __forceinline__ void put(int offset, int piece, uint4 v) const {
+    const int at = ROW_BYTES == 64 ? piece ^ ((lane >> 1) & 3) : piece ^ (lane & 7);
+    *reinterpret_cast<uint4*>(base + offset + lane * ROW_BYTES + at * 16) = v;
+  }
+  __device__ __forceinline__ void written() const {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  }
+  __device__ __forceinline__ void store(const CUtensorMap* map, int offset, int x, int y) const {
+    if (lane == 0)
+      asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                   "r"(smem_u32(base + offset)), "r"(x), "r"(y)
+                   : "memory");
+  }
+  __device__ __forceinline__ void add(const CUtensorMap* map, int offset, int x, int y) const {
+    if (lane == 0)
+      asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map),
+                   "r"(smem_u32(base + offset)), "r"(x), "r"(y)
+                   : "memory");
+  }
+  __device__ __forceinline__ void end() const {
+    if (lane == 0) asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void finish() const {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+};
+
+__device__ __forceinline__ uint4 pack_bf16(const float* x) {
+  uint4 v;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+    w[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return v;
+}
+
+// The rows of a tile, one thread each: 32 columns at a time.
 template <int PARTS, int EPI>
 struct RowEpilogue {
+  const Maps& maps;
   const Args& e;
-  int row;                  // row of the product
-  bool live;                // it exists
-  int job, split;
-  // kStats
-  float top, sum;
+  const BlockOut& out;
+  const Tile& t;
+  int row, first_row;       // of the product: this thread's, the warp's first
+  bool live;                // the row exists
   int target;
-  // kGrad
-  float lse2, c;
-  // scale of the accumulators
-  float factor;
+  float factor;             // of the accumulators
+  float top, sum;           // kStats
+  float lse2, c;            // kGrad
 
-  __device__ __forceinline__ RowEpilogue(const Args& args, const Tile& t, int row_in_tile, int kept) : e(args) {
-    row = t.m * kTile + row_in_tile;
-    job = t.job;
-    split = t.split;
+  __device__ __forceinline__ RowEpilogue(const Maps& maps_, const Args& args, const BlockOut& out_, const Tile& tile,
+                                         int warp_row, int kept)
+      : maps(maps_), e(args), out(out_), t(tile) {
+    first_row = t.m * kTile + warp_row;
+    row = first_row + out.lane;
     factor = 1.f;
     if constexpr (EPI == kGradients) {
-      live = row < (job == 0 ? kept : e.width);
-      if (PARTS == 2 && job == 1) {
+      if (PARTS == 2 && t.job == 1) {
         factor = power_of_two(-14 - scale_exponent(*e.dw_rows_largest));
         if (e.dw_factor != nullptr && kept > 0) factor *= *e.dw_factor;
       }
@@ -485,64 +535,48 @@ struct RowEpilogue {
     } else if constexpr (EPI == kGrad) {
       const int at = target - e.v0 - col;
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float p = exp2_fast(fmaf(v[j], kLog2e, -lse2));
-        v[j] = p;
-      }
+      for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -lse2));
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (at == j) v[j] -= 1.f;
       }
-      const int64_t to = (int64_t)row * e.g_ld + col;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = live ? c * v[j] : 0.f;
+      out.begin();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = live ? c * v[8 * q + j] : 0.f;
         if constexpr (PARTS == 2) {
-          store_parts(x, static_cast<__half*>(e.g[0]) + to + 8 * q, static_cast<__half*>(e.g[1]) + to + 8 * q);
+          __align__(16) __half hi[8], lo[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) split(v[8 * q + j], hi[j], lo[j]);
+          out.put<64>(0, q, *reinterpret_cast<const uint4*>(hi));
+          out.put<64>(kOutBytes / 2, q, *reinterpret_cast<const uint4*>(lo));
         } else {
-          store8(static_cast<__nv_bfloat16*>(e.g[0]) + to + 8 * q, x);
+          out.put<64>(0, q, pack_bf16(v + 8 * q));
         }
       }
+      out.written();
+      out.store(&maps.out[0], 0, col, first_row);
+      if (PARTS == 2) out.store(&maps.out[1], kOutBytes / 2, col, first_row);
+      out.end();
     } else {
-      if (!live) return;
+      if (col >= e.d || (t.job == 1 && first_row >= e.width)) return;
+      out.begin();
+      if (PARTS == 2 || t.job == 0) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (col + 8 * q >= e.d) break;       // d is a multiple of 8
-        float x[8];
+        for (int q = 0; q < 8; ++q)
+          out.put<128>(0, q, *reinterpret_cast<const uint4*>(v + 4 * q));
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = v[8 * q + j];
-        if (job == 0) {
-          float4* to = reinterpret_cast<float4*>(e.slots + (split * e.n_pad + row) * e.d + col + 8 * q);
-          float4 a = make_float4(x[0], x[1], x[2], x[3]), b = make_float4(x[4], x[5], x[6], x[7]);
-          if (e.add) {
-            const float4 a0 = to[0], b0 = to[1];
-            a = make_float4(a.x + a0.x, a.y + a0.y, a.z + a0.z, a.w + a0.w);
-            b = make_float4(b.x + b0.x, b.y + b0.y, b.z + b0.z, b.w + b0.w);
-          }
-          to[0] = a;
-          to[1] = b;
-        } else {
-          const int64_t to = (int64_t)(e.v0 + row) * e.d + col + 8 * q;
-          if constexpr (PARTS == 2) {
-            float4* f = reinterpret_cast<float4*>(static_cast<float*>(e.dw) + to);
-            f[0] = make_float4(x[0], x[1], x[2], x[3]);
-            f[1] = make_float4(x[4], x[5], x[6], x[7]);
-          } else {
-            store8(static_cast<__nv_bfloat16*>(e.dw) + to, x);
-          }
-        }
+        for (int q = 0; q < 4; ++q) out.put<64>(0, q, pack_bf16(v + 8 * q));
       }
+      out.written();
+      if (t.job == 1) out.store(&maps.out[1], 0, col, e.v0 + first_row);
+      else if (e.add) out.add(&maps.out[0], 0, col, t.split * (int)e.n_pad + first_row);
+      else out.store(&maps.out[0], 0, col, t.split * (int)e.n_pad + first_row);
+      out.end();
     }
-  }
-
-  __device__ __forceinline__ static void store8(__nv_bfloat16* to, const float (&x)[8]) {
-    __align__(16) __nv_bfloat162 h[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(h);
   }
 
   __device__ __forceinline__ void finish(int column_part) {
@@ -674,10 +708,10 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
   constexpr int STAGES = Stages<PARTS>::kCount;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + STAGES * Stages<PARTS>::kBytes);   // used in the leader
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStageBytes + kEpilogueWarps * kOutBytes);   // used in the leader
   uint64_t* empty = full + STAGES;
   uint64_t* tfull = empty + STAGES;
-  uint64_t* tempty = tfull + 2;                                                          // used in the leader
+  uint64_t* tempty = tfull + 2;                                                                    // used in the leader
   uint64_t* done = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -762,14 +796,15 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
     // ---------------- epilogue: a TMEM lane (row) per thread, two warps per lane quarter sharing the columns ----------
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
-    const int row_in_tile = (int)rank * 128 + quarter * 32 + lane;
+    const int warp_row = (int)rank * 128 + quarter * 32;
+    const BlockOut block{smem + kStageBytes + (warp - 2) * kOutBytes, lane};
     const uint32_t release[2] = {at_leader(&tempty[0]), at_leader(&tempty[1])};
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     for (int index = pair; index < tiles && ok; index += pairs) {
       const Tile t = tile_of<EPI>(index, extent, e);
-      RowEpilogue<PARTS, EPI> out(e, t, row_in_tile, kept);
+      RowEpilogue<PARTS, EPI> out(maps, e, block, t, warp_row, kept);
       const int col = t.n * kTile + half * 128;
       if constexpr (PARTS == 2) {
         float total[128];
@@ -834,6 +869,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
       }
       out.finish(2 * t.n + half);
     }
+    block.finish();
     if (!ok) {
       if (lane == 0) atomicCAS(&g_error, 0, kErrEpilogue);
       *abort_flag = 1;
@@ -968,27 +1004,38 @@ static int hidden_splits(int dtype, int64_t n, int d, int vocab) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, 74 / tiles));
 }
 
-static int make_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t columns, int64_t ld,
-                    int box_rows) {
+// A row-major matrix in boxes of box_columns x box_rows; the swizzle is that of a box row's bytes (64 or 128).
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t columns, int64_t ld,
+                    int box_columns, int box_rows) {
   auto fn = encode_fn();
   if (fn == nullptr) {
     set_error("cuTensorMapEncodeTiled unavailable");
     return HFFN_ERR_CUDA;
   }
+  const int element = type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
-  const cuuint32_t box[2] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows};
-  const cuuint32_t element[2] = {1, 1};
-  const CUtensorMapDataType type = dtype == HFFN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, element, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * element)};
+  const cuuint32_t box[2] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows};
+  const cuuint32_t step[2] = {1, 1};
+  const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        box_columns * element == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (%d) for a [%lld, %lld] operand", (int)r, (long long)rows,
               (long long)columns);
     return HFFN_ERR_CUDA;
   }
   return HFFN_OK;
+}
+
+static CUtensorMapDataType part_type(int dtype) {
+  return dtype == HFFN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+// An operand part (fp16 or bfloat16) in boxes of 64 columns (K-major: k, 128 rows; MN-major: m or n, 64 rows of k).
+static int operand_map(CUtensorMap* map, int dtype, const void* base, int64_t rows, int64_t columns, int64_t ld,
+                       int box_rows) {
+  return make_map(map, part_type(dtype), base, rows, columns, ld, kBlockK, box_rows);
 }
 
 template <int PARTS, int EPI>
@@ -1014,8 +1061,8 @@ static int launch_products(const Maps& maps, const Args& e, int64_t most_tiles, 
 static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_t n, int d, int vocab) {
   const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
   for (int part = 0; part < parts_of(dtype); ++part) {
-    HFFN_TRY(make_map(&maps.a[0][part], dtype, e.s.hidden[part], e.n_pad, d, d, 128));
-    HFFN_TRY(make_map(&maps.b[0][part], dtype, head[part], vocab, d, d, 128));
+    HFFN_TRY(operand_map(&maps.a[0][part], dtype, e.s.hidden[part], e.n_pad, d, d, 128));
+    HFFN_TRY(operand_map(&maps.b[0][part], dtype, head[part], vocab, d, d, 128));
   }
   e.job[0] = {(int)n, e.width, d, 0, 1, e.v0};
   e.job[1] = {};
@@ -1120,11 +1167,6 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
   e.vocab = vocab;
   e.n_pad = round_up(n, kTile);
   e.upstream = w.upstream;
-  e.g[0] = w.g[0];
-  e.g[1] = w.g[1];
-  e.g_ld = width;
-  e.slots = w.slots;
-  e.dw = grad_weight;
   upstream_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(e.s, grad_loss, reduction, w.upstream);
   const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
   if (PARTS == 2) {
@@ -1151,15 +1193,18 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
     const int64_t columns = ceil_div(e.width, kTile);
     Maps maps;
     HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
+    for (int part = 0; part < PARTS; ++part)
+      HFFN_TRY(make_map(&maps.out[part], part_type(dtype), w.g[part], e.n_pad, width, width, 32, 32));
     HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, st)));
     e.jobs = 0;
     int64_t tiles = 0;
     if (grad_hidden != nullptr) {
       const int j = e.jobs++;
       for (int part = 0; part < PARTS; ++part) {
-        HFFN_TRY(make_map(&maps.a[j][part], dtype, w.g[part], e.n_pad, e.width, width, 128));
-        HFFN_TRY(make_map(&maps.b[j][part], dtype, head[part], vocab, d, d, kBlockK));
+        HFFN_TRY(operand_map(&maps.a[j][part], dtype, w.g[part], e.n_pad, e.width, width, 128));
+        HFFN_TRY(operand_map(&maps.b[j][part], dtype, head[part], vocab, d, d, kBlockK));
       }
+      HFFN_TRY(make_map(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, w.slots, splits * e.n_pad, d, d, 32, 32));
       e.job[j] = {n, d, e.width, 0, splits, v0};
       tiles += row_tiles * wide * splits;
     }
@@ -1167,9 +1212,11 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       // job 1 is dw: without dh, job 0 is empty
       if (e.jobs == 0) e.job[e.jobs++] = {};
       for (int part = 0; part < PARTS; ++part) {
-        HFFN_TRY(make_map(&maps.a[1][part], dtype, w.g[part], e.n_pad, e.width, width, kBlockK));
-        HFFN_TRY(make_map(&maps.b[1][part], dtype, rows[part], e.n_pad, d, d, kBlockK));
+        HFFN_TRY(operand_map(&maps.a[1][part], dtype, w.g[part], e.n_pad, e.width, width, kBlockK));
+        HFFN_TRY(operand_map(&maps.b[1][part], dtype, rows[part], e.n_pad, d, d, kBlockK));
       }
+      HFFN_TRY(make_map(&maps.out[1], PARTS == 2 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        grad_weight, vocab, d, d, 32, 32));
       e.job[1] = {e.width, d, n, 2, 1, 0};
       e.jobs = 2;
       tiles += columns * wide;
