@@ -162,3 +162,10 @@ def check(status: int, what: str) -> None:
 def stream_handle(device) -> int:
     import torch
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def on_device(index: int):
+    """A context in which CUDA device ``index`` is current (nothing to do when it already is)."""
+    import torch
+    from contextlib import nullcontext
+    return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)

@@ -58,6 +58,7 @@ __host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return (a + 
 // What the forward leaves for the backward, in one buffer.
 struct State {
   int32_t* kept;       // [1] rows kept
+  uint32_t* arrived;   // [1] blocks of the losses that are done
   uint32_t* largest;   // [2] float32: bits of the largest finite |entry| of the kept rows and of the head
   int32_t* row_of;     // [n] the input row of each kept row
   int32_t* place_of;   // [n] the kept row of each input row; -1: left out
@@ -84,7 +85,8 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   const int64_t n_pad = round_up(n, kTile);
   State s = {};
   s.kept = c.take<int32_t>(4);
-  s.largest = reinterpret_cast<uint32_t*>(s.kept + 1);
+  s.arrived = reinterpret_cast<uint32_t*>(s.kept + 1);
+  s.largest = reinterpret_cast<uint32_t*>(s.kept + 2);
   s.row_of = c.take<int32_t>(n_pad);
   s.place_of = c.take<int32_t>(n_pad);
   s.target = c.take<int32_t>(n_pad);
@@ -95,6 +97,16 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   s.bytes = c.at;
   return s;
 }
+
+// The gradient of the losses as the caller gave it: c_t of a kept row.
+struct Upstream {
+  const float* grad_loss;
+  int reduction;
+  __device__ __forceinline__ float of(const State& s, int row, int kept) const {
+    if (reduction == HFFN_REDUCE_NONE) return grad_loss[s.row_of[row]];
+    return reduction == HFFN_REDUCE_MEAN ? grad_loss[0] / (float)kept : grad_loss[0];
+  }
+};
 
 // ---- scales of the fp16 parts -------------------------------------------------------------------------------------
 // The exponent e of an operand's scale 2^e from the bits of its largest finite magnitude.
@@ -151,8 +163,8 @@ __device__ __forceinline__ void raise_largest(uint32_t* largest, uint32_t bits) 
 
 // Blocks [0, gather): a block owns `span` consecutive input rows. It counts the kept rows before them (from the targets
 // alone, so that no block waits for another), places its own, and copies them (bfloat16) or raises the largest
-// magnitude by theirs (float32; a second kernel stores the parts). The last block zeroes the kept rows up to a whole
-// stage of K of the dw product. The other blocks (float32) raise the largest magnitude of the head.
+// magnitude by theirs (float32; a second kernel stores the parts). The other blocks (float32) raise the largest
+// magnitude of the head.
 template <typename T>
 __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden, int64_t stride, const T* head,
                                                                 const int64_t* targets, int64_t ignore, int n, int d,
@@ -165,11 +177,18 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
     const float4* from = reinterpret_cast<const float4*>(head);
     const int64_t count = (int64_t)vocab * d / 4, step = (int64_t)(gridDim.x - gather) * kGatherThreads;
     uint32_t bits = 0;
-#pragma unroll 4
-    for (int64_t i = (int64_t)(blockIdx.x - gather) * kGatherThreads + threadIdx.x; i < count; i += step) {
-      const float4 x = from[i];
+    auto raise = [&](float4 x) {
       bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
+    };
+    int64_t i = (int64_t)(blockIdx.x - gather) * kGatherThreads + threadIdx.x;
+    for (; i + 7 * step < count; i += 8 * step) {
+      float4 x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = from[i + j * step];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) raise(x[j]);
     }
+    for (; i < count; i += step) raise(from[i]);
     raise_largest(s.largest + 1, bits);
     return;
   }
@@ -212,12 +231,9 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
     place += __popc(mask);
   }
   if (kF32) raise_largest(s.largest, bits);
-  if (last == n) {
-    if (threadIdx.x == 0) *s.kept = place;
-    const int64_t end = round_up(place, kBlockK) * d / 8;
-    for (int part = 0; part < (kF32 ? 2 : 1); ++part)
-      for (int64_t i = (int64_t)place * d / 8 + threadIdx.x; i < end; i += kGatherThreads)
-        static_cast<uint4*>(s.hidden[part])[i] = make_uint4(0, 0, 0, 0);
+  if (last == n && threadIdx.x == 0) {
+    *s.kept = place;
+    *s.arrived = 0;
   }
 }
 
@@ -251,12 +267,12 @@ __global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t
 // float32, a gradient of its own for each token: rows c_t h_t of the kept rows, first their largest magnitude, then
 // their fp16 parts (padded with zeros to a whole stage of K).
 template <bool kStore>
-__global__ void __launch_bounds__(256) scaled_rows_kernel(State s, const float* upstream, uint32_t* largest, __half* hi,
+__global__ void __launch_bounds__(256) scaled_rows_kernel(State s, Upstream upstream, uint32_t* largest, __half* hi,
                                                           __half* lo, int d) {
   const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), kept = *s.kept;
   if (row >= (kStore ? (int)round_up(kept, kBlockK) : kept)) return;
   const float inverse = power_of_two(-scale_exponent(s.largest[0]));
-  const float c = row < kept ? upstream[row] : 0.f;
+  const float c = row < kept ? upstream.of(s, row, kept) : 0.f;
   const float scale = kStore ? power_of_two(scale_exponent(*largest)) : 1.f;
   const __half* from_hi = static_cast<const __half*>(s.hidden[0]) + (int64_t)row * d;
   const __half* from_lo = static_cast<const __half*>(s.hidden[1]) + (int64_t)row * d;
@@ -303,10 +319,10 @@ struct Args {
   int64_t n_pad;
   float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials
   float* picked;           // kStats: [n_pad] the target's logit
-  const float* upstream;   // [n_pad] c_t by kept row
+  Upstream upstream;
   int add;                 // kGradients: dh adds to its slots (a later piece)
   const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
-  const float* dw_factor;            // float32: one c for all rows, or NULL
+  int dw_upstream;                   // float32: dw's rows lack their c, which is the same for all
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -490,7 +506,7 @@ struct RowEpilogue {
     if constexpr (EPI == kGradients) {
       if (PARTS == 2 && t.job == 1) {
         factor = power_of_two(-14 - scale_exponent(*e.dw_rows_largest));
-        if (e.dw_factor != nullptr && kept > 0) factor *= *e.dw_factor;
+        if (e.dw_upstream && kept > 0) factor *= e.upstream.of(e.s, 0, kept);
       }
     } else {
       live = row < kept;
@@ -500,7 +516,7 @@ struct RowEpilogue {
       sum = 0.f;
       if (EPI == kGrad) {
         lse2 = live ? e.s.lse[row] * kLog2e : 0.f;
-        c = PARTS == 2 ? 16384.f : live ? e.upstream[row] : 0.f;
+        c = PARTS == 2 ? 16384.f : live ? e.upstream.of(e.s, row, kept) : 0.f;
       }
     }
   }
@@ -894,68 +910,80 @@ __device__ __forceinline__ void merge(float& top, float& sum, float top2, float 
   top = most;
 }
 
+// The block that finishes last also adds up the losses where their sum or mean is asked for (float64, the same order
+// whichever block that is). The blocks after the `row_blocks` zero the kept rows up to a whole stage of K of the dw
+// product.
 __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* stats, int64_t n_pad, int parts,
-                                                      const float* picked, float* losses) {
+                                                      const float* picked, float* losses, int n, int reduction,
+                                                      float* loss, int row_blocks, int row_bytes, int operands) {
   __shared__ float2 shared[32][33];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane, kept = *s.kept;
-  if (blockIdx.x * 32 >= kept) return;
-  float top = -INFINITY, sum = 0.f;
-  if (row < kept) {
-#pragma unroll 4
-    for (int i = warp; i < parts; i += 32) {
-      const float2 v = stats[i * n_pad + row];
-      merge(top, sum, v.x, v.y);
+  if (blockIdx.x >= row_blocks) {
+    const int64_t step = (int64_t)(gridDim.x - row_blocks) * 1024, end = round_up(kept, kBlockK) * row_bytes / 16;
+    for (int part = 0; part < operands; ++part)
+      for (int64_t i = (int64_t)kept * row_bytes / 16 + (blockIdx.x - row_blocks) * 1024 + threadIdx.x; i < end;
+           i += step)
+        static_cast<uint4*>(s.hidden[part])[i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  if (blockIdx.x * 32 < kept) {
+    float top = -INFINITY, sum = 0.f;
+    if (row < kept) {
+      for (int i = warp; i < parts; i += 256) {
+        float2 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[j] = i + 32 * j < parts ? stats[(i + 32 * j) * n_pad + row] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) merge(top, sum, v[j].x, v[j].y);
+      }
+    }
+    shared[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    float2 v = shared[lane][warp];           // row `warp` of the block, one part a lane
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float top2 = __shfl_xor_sync(0xffffffffu, v.x, o), sum2 = __shfl_xor_sync(0xffffffffu, v.y, o);
+      merge(v.x, v.y, top2, sum2);
+    }
+    const int mine = blockIdx.x * 32 + warp;
+    if (lane == 0 && mine < kept) {
+      const float lse = v.x + logf(v.y);
+      s.lse[mine] = lse;
+      losses[s.row_of[mine]] = lse - picked[mine];
     }
   }
-  shared[warp][lane] = make_float2(top, sum);
+  if (reduction == HFFN_REDUCE_NONE) return;
+  __shared__ bool last;
+  __threadfence();
   __syncthreads();
-  float2 v = shared[lane][warp];           // row `warp` of the block, one part a lane
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float top2 = __shfl_xor_sync(0xffffffffu, v.x, o), sum2 = __shfl_xor_sync(0xffffffffu, v.y, o);
-    merge(v.x, v.y, top2, sum2);
-  }
-  const int mine = blockIdx.x * 32 + warp;
-  if (lane == 0 && mine < kept) {
-    const float lse = v.x + logf(v.y);
-    s.lse[mine] = lse;
-    losses[s.row_of[mine]] = lse - picked[mine];
-  }
-}
-
-// The sum or the mean of the rows' losses (float64, a fixed order): one block.
-__global__ void __launch_bounds__(1024) reduce_kernel(State s, const float* losses, int n, int mean, float* loss) {
-  __shared__ double shared[32];
+  if (threadIdx.x == 0) last = atomicAdd(s.arrived, 1u) == (unsigned)row_blocks - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double* sums = reinterpret_cast<double*>(shared);
   double sum = 0;
-  for (int t = threadIdx.x; t < n; t += 1024) sum += (double)losses[t];
+  for (int t = threadIdx.x; t < n; t += 1024) sum += (double)__ldcg(losses + t);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = sum;
+  if (lane == 0) sums[warp] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0;
-    for (int w = 0; w < 32; ++w) sum += shared[w];
-    *loss = (float)(mean ? sum / max(1, *s.kept) : sum);
+    for (int w = 0; w < 32; ++w) sum += sums[w];
+    *loss = (float)(reduction == HFFN_REDUCE_MEAN ? sum / max(1, kept) : sum);
   }
-}
-
-// c_t of each kept row.
-__global__ void __launch_bounds__(256) upstream_kernel(State s, const float* grad_loss, int reduction, float* upstream) {
-  const int at = blockIdx.x * 256 + threadIdx.x, kept = *s.kept;
-  if (at >= kept) return;
-  upstream[at] = reduction == HFFN_REDUCE_NONE ? grad_loss[s.row_of[at]]
-                 : reduction == HFFN_REDUCE_MEAN ? grad_loss[0] / (float)kept : grad_loss[0];
 }
 
 // dh of each input row: the sum of its kept row's slots (in order), or zeros. One warp a row.
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(State s, const float* slots, int splits, int64_t n_pad,
-                                                      const float* upstream, T* grad_hidden, int n, int d) {
+                                                      Upstream upstream, T* grad_hidden, int n, int d) {
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t >= n) return;
   const int at = s.place_of[t];
   float factor = 1.f;
-  if (sizeof(T) == 4 && at >= 0) factor = upstream[at] * power_of_two(-14 - scale_exponent(s.largest[1]));
+  if (sizeof(T) == 4 && at >= 0) factor = upstream.of(s, at, *s.kept) * power_of_two(-14 - scale_exponent(s.largest[1]));
   for (int i = 4 * lane; i < d; i += 128) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= 0)
@@ -1005,8 +1033,8 @@ static int hidden_splits(int dtype, int64_t n, int d, int vocab) {
 }
 
 // A row-major matrix in boxes of box_columns x box_rows; the swizzle is that of a box row's bytes (64 or 128).
-static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t columns, int64_t ld,
-                    int box_columns, int box_rows) {
+static int make_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t columns,
+                    int64_t ld, int box_columns, int box_rows) {
   auto fn = encode_fn();
   if (fn == nullptr) {
     set_error("cuTensorMapEncodeTiled unavailable");
@@ -1088,7 +1116,6 @@ static ForwardWork forward_work(void* base, int64_t n, int vocab) {
 }
 
 struct BackwardWork {
-  float* upstream;
   void* g[2];
   float* slots;
   uint32_t* largest;      // float32, a gradient for each token: of c h
@@ -1100,7 +1127,6 @@ static BackwardWork backward_work(void* base, int dtype, int64_t n, int d, int v
   Carve c{static_cast<uint8_t*>(base)};
   const int64_t n_pad = round_up(n, kTile);
   BackwardWork w = {};
-  w.upstream = c.take<float>(n_pad);
   for (int part = 0; part < parts_of(dtype); ++part) w.g[part] = c.take<uint16_t>(n_pad * piece_width(dtype, n, vocab));
   w.slots = c.take<float>(hidden_splits(dtype, n, d, vocab) * n_pad * d);
   if (dtype == HFFN_F32) {
@@ -1147,10 +1173,9 @@ static int forward(const void* hidden, int64_t stride, const void* weight, const
   Maps maps;
   HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
   HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), st)));
-  losses_kernel<<<(unsigned)ceil_div(n, 32), 1024, 0, st>>>(e.s, w.stats, e.n_pad, 2 * (int)ceil_div(vocab, kTile),
-                                                           w.picked, losses);
-  if (reduction != HFFN_REDUCE_NONE)
-    reduce_kernel<<<1, 1024, 0, st>>>(e.s, losses, n, reduction == HFFN_REDUCE_MEAN, loss);
+  const int row_blocks = (int)ceil_div(n, 32);
+  losses_kernel<<<row_blocks + 4, 1024, 0, st>>>(e.s, w.stats, e.n_pad, 2 * (int)ceil_div(vocab, kTile), w.picked, losses,
+                                                 n, reduction, loss, row_blocks, 2 * d, PARTS);
   return launch_status("linear_ce_forward");
 }
 
@@ -1166,13 +1191,12 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
   e.d = d;
   e.vocab = vocab;
   e.n_pad = round_up(n, kTile);
-  e.upstream = w.upstream;
-  upstream_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, st>>>(e.s, grad_loss, reduction, w.upstream);
+  e.upstream = {grad_loss, reduction};
   const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
   if (PARTS == 2) {
     e.dw_rows_largest = e.s.largest;
     if (reduction != HFFN_REDUCE_NONE) {
-      e.dw_factor = w.upstream;
+      e.dw_upstream = 1;
     } else if (grad_weight != nullptr) {
       e.dw_rows_largest = w.largest;
       rows[0] = w.rows[0];
@@ -1180,8 +1204,8 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
       __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
       const unsigned blocks = (unsigned)(e.n_pad / 8);
-      scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, w.upstream, w.largest, hi, lo, d);
-      scaled_rows_kernel<true><<<blocks, 256, 0, st>>>(e.s, w.upstream, w.largest, hi, lo, d);
+      scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
+      scaled_rows_kernel<true><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
     }
   }
   const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
@@ -1224,9 +1248,22 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
     if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, st)));
   }
   if (grad_hidden != nullptr)
-    scatter_kernel<T><<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(e.s, w.slots, splits, e.n_pad, w.upstream,
+    scatter_kernel<T><<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(e.s, w.slots, splits, e.n_pad, e.upstream,
                                                                 static_cast<T*>(grad_hidden), n, d);
   return launch_status("linear_ce_backward");
+}
+
+// Makes the current device's context current for the calling thread too, where that has made no CUDA call yet (a
+// framework's backward thread): the tensor maps are encoded by the driver, which asks for one.
+static int bind_context() {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess) e = cudaSetDevice(device);
+  if (e != cudaSuccess) {
+    set_error("linear_ce: %s", cudaGetErrorString(e));
+    return HFFN_ERR_CUDA;
+  }
+  return HFFN_OK;
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1264,6 +1301,7 @@ int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride,
   HFFN_REQUIRE(ce::aligned16(weight) && ce::aligned16(state) && ce::aligned16(work),
                "weight, state and work must be 16-byte aligned");
   HFFN_TRY(bind_stream_device(stream));
+  HFFN_TRY(ce::bind_context());
   auto run = dtype == HFFN_F32 ? ce::forward<float> : ce::forward<__nv_bfloat16>;
   return run(hidden, hidden_stride, weight, targets, ignore_index, reduction, loss, state, work, (int)n, d, vocab,
              static_cast<cudaStream_t>(stream));
@@ -1280,6 +1318,7 @@ int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const 
                    ce::aligned16(grad_weight),
                "weight, gradients, state and work must be 16-byte aligned");
   HFFN_TRY(bind_stream_device(stream));
+  HFFN_TRY(ce::bind_context());
   auto run = dtype == HFFN_F32 ? ce::backward<float> : ce::backward<__nv_bfloat16>;
   return run(weight, reduction, grad_loss, grad_hidden, grad_weight, state, work, (int)n, d, vocab,
              static_cast<cudaStream_t>(stream));

@@ -7,19 +7,19 @@ gradients; these functions take any list of float32 and bfloat16 CUDA tensors.
 """
 from __future__ import annotations
 
-import ctypes
+from array import array
 
 import torch
 
 from . import _native as native
 
-DTYPES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
+_CODES = {torch.float32: native.F32, torch.bfloat16: native.BF16}
 
 
 def _dense(t: torch.Tensor) -> bool:
     """Whether the tensor's entries fill one stretch of memory, each once (contiguous, or a permutation of it)."""
-    if t.is_contiguous():
-        return True
+    if t.layout != torch.strided:
+        return False
     expected = 1
     for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
         if stride != expected:
@@ -28,67 +28,80 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _check(tensors, what: str) -> list[torch.Tensor]:
-    tensors = list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.dtype not in DTYPES or t.layout != torch.strided:
-            raise ValueError(f"{what} must be float32 or bfloat16 tensors")
-        if not t.is_cuda or t.device != tensors[0].device:
+class _List:
+    """A checked list of tensors and the host arrays of the native calls. Written as passes of C-level calls over the
+    list: a model has hundreds of gradients, and this is the host's cost of a call."""
+
+    def __init__(self, tensors, what: str) -> None:
+        tensors = self.tensors = list(tensors)
+        try:
+            types = [_CODES[t.dtype] for t in tensors]
+            devices = set(map(torch.Tensor.get_device, tensors))
+            self.contiguous = list(map(torch.Tensor.is_contiguous, tensors))
+            if not all(self.contiguous) and not all(c or _dense(t) for c, t in zip(self.contiguous, tensors)):
+                raise ValueError(f"{what} must be dense in memory")
+            self.pointers = array("Q", map(torch.Tensor.data_ptr, tensors))
+            self.counts = array("q", map(torch.Tensor.numel, tensors))
+        except (KeyError, TypeError, AttributeError, RuntimeError):
+            raise ValueError(f"{what} must be dense float32 or bfloat16 tensors") from None
+        if len(devices) > 1 or -1 in devices:
             raise ValueError(f"{what} must be on one CUDA device")
-        if not _dense(t):
-            raise ValueError(f"{what} must be dense in memory")
-    return tensors
+        self.types = array("i", types)
+        self.device = devices.pop() if devices else torch.cuda.current_device()
+
+    def __len__(self) -> int:
+        return len(self.tensors)
 
 
-def _arrays(tensors):
-    count = len(tensors)
-    return ((ctypes.c_void_p * count)(*[t.data_ptr() for t in tensors]),
-            (ctypes.c_int64 * count)(*[t.numel() for t in tensors]),
-            (ctypes.c_int32 * count)(*[DTYPES[t.dtype] for t in tensors]))
+def _address(a: array) -> int:
+    return a.buffer_info()[0]
 
 
-def _buffers(tensors):
+def _buffers(tensors: _List):
     """The norm (a float32 scalar) and the workspace of a call, from torch's allocator on the current stream."""
-    device = tensors[0].device if tensors else torch.device("cuda", torch.cuda.current_device())
-    size = int(native.lib.hffn_grad_norm_workspace(len(tensors)))
-    return device, torch.empty((), device=device), torch.empty(size, dtype=torch.uint8, device=device)
+    device = torch.device("cuda", tensors.device)
+    size = native.lib.hffn_grad_norm_workspace(len(tensors))
+    return torch.empty((), device=device), torch.empty(size, dtype=torch.uint8, device=device)
 
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm over every entry of ``tensors`` (float32 / bfloat16, dense, on one CUDA device): a float32 scalar on
     that device, computed in float64 and rounded once. An empty list has norm 0 (on the current device)."""
-    tensors = _check(tensors, "tensors")
-    device, norm, work = _buffers(tensors)
-    pointers, counts, types = _arrays(tensors)
-    with torch.cuda.device(device):
-        native.check(native.lib.hffn_grad_norm(len(tensors), pointers, counts, types, norm.data_ptr(), work.data_ptr(),
-                                               native.stream_handle(device)), "hffn_grad_norm")
+    tensors = _List(tensors, "tensors")
+    norm, work = _buffers(tensors)
+    with native.on_device(tensors.device):
+        native.check(native.lib.hffn_grad_norm(len(tensors), _address(tensors.pointers), _address(tensors.counts),
+                                               _address(tensors.types), norm.data_ptr(), work.data_ptr(),
+                                               native.stream_handle(tensors.device)), "hffn_grad_norm")
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
     """Scale every entry by ``min(1, max_norm / (norm + 1e-6))`` and return the norm before it (``grad_norm``), a
     float32 scalar on the device; the host waits for nothing.
 
-    In place, or into ``out``: one tensor of the same shape for each (float32 or bfloat16, e.g. an optimizer's float32
-    buffers for bfloat16 gradients). The scaled values are computed in float32 and rounded once to the output's type.
+    In place, or into ``out``: one tensor for each (float32 or bfloat16, e.g. an optimizer's float32 buffers for bfloat16
+    gradients), contiguous with as many entries, or of the same shape and strides. The scaled values are computed in
+    float32 and rounded once to the output's type.
     With a norm that is infinite or NaN the factor is 0 or NaN, as with ``torch.nn.utils.clip_grad_norm_``.
     Refused (ValueError): tensors that share memory with one that is written, an output that overlaps another tensor's
     input, a negative ``max_norm``."""
-    tensors = _check(tensors, "tensors")
-    outs = tensors if out is None else _check(out, "outputs")
-    if len(outs) != len(tensors) or any(o.shape != t.shape or (o is not t and o.stride() != t.stride())
-                                        for o, t in zip(outs, tensors)):
-        raise ValueError("out needs one tensor of the same shape and strides for each")
-    if tensors and outs[0].device != tensors[0].device:
-        raise ValueError("outputs must be on the tensors' device")
-    device, norm, work = _buffers(tensors)
-    pointers, counts, types = _arrays(tensors)
-    out_pointers, _, out_types = _arrays(outs)
-    with torch.cuda.device(device):
-        native.check(native.lib.hffn_clip_grad_norm(len(tensors), pointers, out_pointers, counts, types, out_types,
-                                                    float(max_norm), norm.data_ptr(), work.data_ptr(),
-                                                    native.stream_handle(device)), "hffn_clip_grad_norm")
-    torch.autograd.graph.increment_version(outs)
+    tensors = _List(tensors, "tensors")
+    outs = tensors if out is None else _List(out, "outputs")
+    if outs is not tensors:
+        if len(outs) != len(tensors) or outs.counts != tensors.counts:
+            raise ValueError("out needs one tensor with as many entries for each")
+        if len(outs) and outs.device != tensors.device:
+            raise ValueError("outputs must be on the tensors' device")
+        if not all(tensors.contiguous) or not all(outs.contiguous):
+            if any(not (a and b) and (t.shape != o.shape or t.stride() != o.stride()) for a, b, t, o in
+                   zip(tensors.contiguous, outs.contiguous, tensors.tensors, outs.tensors)):
+                raise ValueError("outputs that are not contiguous need their tensor's shape and strides")
+    norm, work = _buffers(tensors)
+    with native.on_device(tensors.device):
+        native.check(native.lib.hffn_clip_grad_norm(
+            len(tensors), _address(tensors.pointers), _address(outs.pointers), _address(tensors.counts),
+            _address(tensors.types), _address(outs.types), float(max_norm), norm.data_ptr(), work.data_ptr(),
+            native.stream_handle(tensors.device)), "hffn_clip_grad_norm")
+    torch.autograd.graph.increment_version(outs.tensors)
     return norm

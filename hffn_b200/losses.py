@@ -7,6 +7,8 @@ Types: float32 and bfloat16 (hidden and weight alike); losses are float32, sums 
 """
 from __future__ import annotations
 
+from functools import lru_cache
+
 import torch
 
 from . import _native as native
@@ -35,8 +37,12 @@ def _check(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
         raise ValueError("unsupported token count")
 
 
-def _bytes(size: int, device) -> torch.Tensor:
-    return torch.empty(size, dtype=torch.uint8, device=device)
+@lru_cache(maxsize=256)
+def _sizes(code: int, n: int, d: int, vocab: int) -> tuple[int, int, int]:
+    """Bytes of the state, the forward's and the backward's workspace."""
+    return (native.lib.hffn_linear_ce_state_bytes(code, n, d, vocab),
+            native.lib.hffn_linear_ce_forward_workspace(code, n, d, vocab),
+            native.lib.hffn_linear_ce_backward_workspace(code, n, d, vocab))
 
 
 def _forward(hidden, weight, targets, ignore_index, reduction):
@@ -46,10 +52,11 @@ def _forward(hidden, weight, targets, ignore_index, reduction):
     if hidden.stride(1) != 1 or (n > 1 and hidden.stride(0) < d):
         hidden = hidden.contiguous()
     targets = targets.contiguous()
+    state_bytes, work_bytes, _ = _sizes(code, n, d, vocab)
     loss = torch.empty(n if reduction == "none" else (), device=device)
-    state = _bytes(native.lib.hffn_linear_ce_state_bytes(code, n, d, vocab), device)
-    work = _bytes(native.lib.hffn_linear_ce_forward_workspace(code, n, d, vocab), device)
-    with torch.cuda.device(device):
+    state = torch.empty(state_bytes, dtype=torch.uint8, device=device)
+    work = torch.empty(work_bytes, dtype=torch.uint8, device=device)
+    with native.on_device(device.index):
         native.check(native.lib.hffn_linear_ce_forward(
             code, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), targets.data_ptr(), ignore_index,
             native.REDUCE_CODES[reduction], loss.data_ptr(), state.data_ptr(), work.data_ptr(), n, d, vocab,
@@ -62,13 +69,12 @@ def _backward(weight, state, n, reduction, grad_loss, want_hidden=True, want_wei
     grad_loss = grad_loss.float().contiguous()
     grad_hidden = torch.empty(n, d, dtype=weight.dtype, device=device) if want_hidden else None
     grad_weight = torch.empty_like(weight) if want_weight else None
-    work = _bytes(native.lib.hffn_linear_ce_backward_workspace(code, n, d, vocab), device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with torch.cuda.device(device):
+    work = torch.empty(_sizes(code, n, d, vocab)[2], dtype=torch.uint8, device=device)
+    with native.on_device(device.index):
         native.check(native.lib.hffn_linear_ce_backward(
-            code, weight.data_ptr(), native.REDUCE_CODES[reduction], grad_loss.data_ptr(), ptr(grad_hidden),
-            ptr(grad_weight), state.data_ptr(), work.data_ptr(), n, d, vocab, native.stream_handle(device)),
-            "hffn_linear_ce_backward")
+            code, weight.data_ptr(), native.REDUCE_CODES[reduction], grad_loss.data_ptr(),
+            grad_hidden.data_ptr() if want_hidden else None, grad_weight.data_ptr() if want_weight else None,
+            state.data_ptr(), work.data_ptr(), n, d, vocab, native.stream_handle(device)), "hffn_linear_ce_backward")
     return grad_hidden, grad_weight
 
 
@@ -105,9 +111,12 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
 
     Arguments are checked before any launch (ValueError). One backward per forward result (no second derivatives)."""
     _check(hidden, weight, targets, reduction)
-    loss = LinearCrossEntropyFunction.apply(hidden.reshape(-1, hidden.shape[-1]), weight, targets.reshape(-1),
-                                            int(ignore_index), reduction)
-    return loss.view(targets.shape) if reduction == "none" else loss
+    rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        loss = LinearCrossEntropyFunction.apply(rows, weight, flat, int(ignore_index), reduction)
+    else:
+        loss, _ = _forward(rows, weight, flat, int(ignore_index), reduction)
+    return loss.view(targets.shape) if reduction == "none" and hidden.dim() != 2 else loss
 
 
 @torch.no_grad()

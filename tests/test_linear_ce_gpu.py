@@ -400,6 +400,18 @@ def test_gradients_outside_autograd(dtype):
         linear_cross_entropy_gradients(h, w, t, c)
 
 
+def test_from_a_thread_that_has_made_no_cuda_call():
+    import threading
+    from hffn_b200.losses import linear_cross_entropy_gradients
+    h, w, t = make(50, 64, 300, torch.float32, seed=23)
+    expected, got = linear_cross_entropy_gradients(h, w, t), []
+    thread = threading.Thread(target=lambda: got.extend(linear_cross_entropy_gradients(h, w, t)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert len(got) == 3 and all(torch.equal(a, b) for a, b in zip(expected, got))
+
+
 def test_a_weight_changed_before_the_backward_is_noticed():
     from hffn_b200.losses import linear_cross_entropy
     h, w, t = make(20, 64, 300, torch.float32)
