@@ -169,3 +169,9 @@ def on_device(index: int):
     import torch
     from contextlib import nullcontext
     return nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(index: int) -> int:
+    """The handle of the current torch stream of CUDA device ``index`` (``stream_handle`` without making a Stream)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(index)

@@ -22,8 +22,8 @@
 // largest keep 22 bits, smaller ones are held to 2^-39 of it. One scale per operand, not per row, because each of h, w
 // and g is summed over its rows in one of the products. g holds 2^14 (p - [v = target]), c_t is applied in float32
 // afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). Sums: the
-// tensor core's float32 accumulation truncates, so float32 results are summed in registers from accumulators of kChunk
-// values of K each.
+// tensor core's float32 accumulation truncates at every step, so what ends in float32 (float32 gradients, losses) is
+// summed in registers from accumulators of few steps each (chunk_of).
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -37,7 +37,6 @@ using namespace tc;
 
 constexpr int kTile = 256;                           // rows and columns of a pair's tile
 constexpr int kBlockK = 64;                          // values of K in a stage: 128 bytes, the swizzle's row
-constexpr int kChunk = 4;                            // stages of K per accumulator (float32)
 constexpr int kThreads = 320;                        // warp 0: loads, warp 1: products, warps 2 to 9: epilogue
 constexpr int kEpilogueWarps = 8;
 constexpr int kGroupRows = 32;                       // row tiles of logits that share their pass over the vocabulary
@@ -66,6 +65,7 @@ struct State {
   float* lse;          // [n]
   void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts)
   void* head[2];       // [vocab, d] float32: the head's fp16 parts
+  float* raw;          // [kFew, d] float32, few rows: the kept rows as they are (their parts are made in the backward)
   int64_t bytes;
 };
 
@@ -79,6 +79,21 @@ struct Carve {
     return p;
   }
 };
+
+// Few float32 rows: their logits are computed on the CUDA cores, straight from the head (few_kernel), where that is
+// faster than making the head's fp16 parts for the tensor cores (two passes over it and one of writes before the
+// products): d 1024, vocabulary 50304, whole calls: 50, 79 and 122 us for 1, 8 and 16 rows against 177; 32 rows would
+// take 228. (bfloat16 has no such detour: 38 us on the tensor cores for 1 to 32 rows, 34 with this kernel for one, 42 for
+// two.) The rows have to fit the kernel's shared memory.
+constexpr int kFewRows = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32;
+constexpr int64_t kFewBytes = 96 << 10;
+
+// Rows of one pass.
+static int few_rows(int64_t n) { return n <= 2 ? (int)n : n <= 4 ? 4 : kFewRows; }
+
+static bool is_few(int dtype, int64_t n, int d) {
+  return dtype == HFFN_F32 && n <= 2 * kFewRows && (int64_t)few_rows(n) * d * 4 <= kFewBytes;
+}
 
 static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   Carve c{static_cast<uint8_t*>(base)};
@@ -94,6 +109,7 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
   if (dtype == HFFN_F32)
     for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
+  if (is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
   s.bytes = c.at;
   return s;
 }
@@ -107,6 +123,14 @@ struct Upstream {
     return reduction == HFFN_REDUCE_MEAN ? grad_loss[0] / (float)kept : grad_loss[0];
   }
 };
+
+// Programmatic dependent launch: a kernel of a call is started while its predecessor still runs (its prologue and its
+// launch then overlap the predecessor's end) and touches global memory only after this, when the predecessor has
+// completed. In a plain launch both are no-ops.
+__device__ __forceinline__ void depend() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
 
 // ---- scales of the fp16 parts -------------------------------------------------------------------------------------
 // The exponent e of an operand's scale 2^e from the bits of its largest finite magnitude.
@@ -161,6 +185,26 @@ __device__ __forceinline__ void raise_largest(uint32_t* largest, uint32_t bits) 
   if ((threadIdx.x & 31) == 0 && bits != 0) atomicMax(largest, bits);
 }
 
+// One block's share of the largest finite magnitude of an array (count a multiple of 4).
+__device__ __forceinline__ uint32_t largest_of(const float* array, int64_t count, int block, int blocks) {
+  const float4* from = reinterpret_cast<const float4*>(array);
+  const int64_t step = (int64_t)blocks * kGatherThreads;
+  uint32_t bits = 0;
+  auto raise = [&](float4 x) {
+    bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
+  };
+  int64_t i = (int64_t)block * kGatherThreads + threadIdx.x;
+  for (; i + 7 * step < count / 4; i += 8 * step) {
+    float4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = from[i + j * step];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) raise(x[j]);
+  }
+  for (; i < count / 4; i += step) raise(from[i]);
+  return bits;
+}
+
 // Blocks [0, gather): a block owns `span` consecutive input rows. It counts the kept rows before them (from the targets
 // alone, so that no block waits for another), places its own, and copies them (bfloat16) or raises the largest
 // magnitude by theirs (float32; a second kernel stores the parts). The other blocks (float32) raise the largest
@@ -172,24 +216,11 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
                                                                 float* losses, State s) {
   constexpr bool kF32 = sizeof(T) == 4;
   __shared__ int shared[kGatherWarps];
+  depend();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (kF32 && blockIdx.x >= gather) {
-    const float4* from = reinterpret_cast<const float4*>(head);
-    const int64_t count = (int64_t)vocab * d / 4, step = (int64_t)(gridDim.x - gather) * kGatherThreads;
-    uint32_t bits = 0;
-    auto raise = [&](float4 x) {
-      bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
-    };
-    int64_t i = (int64_t)(blockIdx.x - gather) * kGatherThreads + threadIdx.x;
-    for (; i + 7 * step < count; i += 8 * step) {
-      float4 x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = from[i + j * step];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) raise(x[j]);
-    }
-    for (; i < count; i += step) raise(from[i]);
-    raise_largest(s.largest + 1, bits);
+    raise_largest(s.largest + 1, largest_of(reinterpret_cast<const float*>(head), (int64_t)vocab * d,
+                                            blockIdx.x - gather, gridDim.x - gather));
     return;
   }
   const int first = blockIdx.x * span, last = min(n, first + span);
@@ -237,21 +268,28 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
   }
 }
 
-// float32: the fp16 parts of the head and of the kept rows, one warp a row.
+// float32: the fp16 parts of the head and of the kept rows (from `hidden`, or from the state where `hidden` is NULL),
+// one warp a row; the kept rows are padded with zeros to a whole stage of K of the dw product.
 __global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t stride, bool aligned, const float* head,
                                                     int d, int vocab, State s) {
-  const int lane = threadIdx.x & 31;
+  depend();
+  const int lane = threadIdx.x & 31, kept = *s.kept;
   int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   const bool of_head = row < vocab;
   if (!of_head) row -= vocab;
-  if (!of_head && row >= *s.kept) return;
+  if (!of_head && row >= (int)round_up(kept, kBlockK)) return;
   const float scale = power_of_two(scale_exponent(s.largest[of_head]));
-  const float* from = of_head ? head + (int64_t)row * d : hidden + (int64_t)s.row_of[row] * stride;
+  const bool zero = !of_head && row >= kept;
+  const float* from = of_head          ? head + (int64_t)row * d
+                      : zero           ? nullptr
+                      : hidden != NULL ? hidden + (int64_t)s.row_of[row] * stride
+                                       : s.raw + (int64_t)row * d;
   __half* hi = static_cast<__half*>(of_head ? s.head[0] : s.hidden[0]) + (int64_t)row * d;
   __half* lo = static_cast<__half*>(of_head ? s.head[1] : s.hidden[1]) + (int64_t)row * d;
   for (int i = 8 * lane; i < d; i += 256) {
-    float x[8];
-    if (of_head || aligned) {
+    float x[8] = {};
+    if (zero) {
+    } else if (of_head || aligned) {
       *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from + i);
       *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(from + i + 4);
     } else {
@@ -264,11 +302,24 @@ __global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t
   }
 }
 
+// float32, few rows, before the backward: the largest magnitudes of the kept rows (block 0) and of the head.
+__global__ void __launch_bounds__(kGatherThreads) measure_kernel(const float* head, int d, int vocab, State s) {
+  depend();
+  uint32_t bits = 0;
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < *s.kept * d; i += kGatherThreads) bits = max(bits, finite_bits(s.raw[i]));
+    raise_largest(s.largest, bits);
+  } else {
+    raise_largest(s.largest + 1, largest_of(head, (int64_t)vocab * d, blockIdx.x - 1, gridDim.x - 1));
+  }
+}
+
 // float32, a gradient of its own for each token: rows c_t h_t of the kept rows, first their largest magnitude, then
 // their fp16 parts (padded with zeros to a whole stage of K).
 template <bool kStore>
 __global__ void __launch_bounds__(256) scaled_rows_kernel(State s, Upstream upstream, uint32_t* largest, __half* hi,
                                                           __half* lo, int d) {
+  depend();
   const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), kept = *s.kept;
   if (row >= (kStore ? (int)round_up(kept, kBlockK) : kept)) return;
   const float inverse = power_of_two(-scale_exponent(s.largest[0]));
@@ -438,10 +489,20 @@ __device__ __forceinline__ Tile tile_of(int index, const Extent (&x)[2], const A
 struct BlockOut {
   uint8_t* base;
   int lane;
+  int half;              // place of the last block
+  bool whole;            // the last block was of 4 KB
 
-  __device__ __forceinline__ void begin() const {      // the last block has been read out
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  // Room for a block of 4 KB, or of 2 KB while another one of 2 KB before it is still read out; its place.
+  template <int BYTES>
+  __device__ __forceinline__ int begin() {
+    if (BYTES == kOutBytes || whole) {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    } else {
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    }
     __syncwarp();
+    whole = BYTES == kOutBytes;
+    return half = whole ? 0 : half ^ (kOutBytes / 2);
   }
   template <int ROW_BYTES>
   __device__ __forceinline__ void put(int offset, int piece, uint4 v) const {
@@ -488,7 +549,7 @@ template <int PARTS, int EPI>
 struct RowEpilogue {
   const Maps& maps;
   const Args& e;
-  const BlockOut& out;
+  BlockOut& out;
   const Tile& t;
   int row, first_row;       // of the product: this thread's, the warp's first
   bool live;                // the row exists
@@ -497,7 +558,7 @@ struct RowEpilogue {
   float top, sum;           // kStats
   float lse2, c;            // kGrad
 
-  __device__ __forceinline__ RowEpilogue(const Maps& maps_, const Args& args, const BlockOut& out_, const Tile& tile,
+  __device__ __forceinline__ RowEpilogue(const Maps& maps_, const Args& args, BlockOut& out_, const Tile& tile,
                                          int warp_row, int kept)
       : maps(maps_), e(args), out(out_), t(tile) {
     first_row = t.m * kTile + warp_row;
@@ -559,36 +620,38 @@ struct RowEpilogue {
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = live ? c * v[j] : 0.f;
-      out.begin();
+      const int at_block = out.template begin<PARTS * kOutBytes / 2>();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if constexpr (PARTS == 2) {
           __align__(16) __half hi[8], lo[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) split(v[8 * q + j], hi[j], lo[j]);
-          out.put<64>(0, q, *reinterpret_cast<const uint4*>(hi));
-          out.put<64>(kOutBytes / 2, q, *reinterpret_cast<const uint4*>(lo));
+          out.template put<64>(0, q, *reinterpret_cast<const uint4*>(hi));
+          out.template put<64>(kOutBytes / 2, q, *reinterpret_cast<const uint4*>(lo));
         } else {
-          out.put<64>(0, q, pack_bf16(v + 8 * q));
+          out.template put<64>(at_block, q, pack_bf16(v + 8 * q));
         }
       }
       out.written();
-      out.store(&maps.out[0], 0, col, first_row);
+      out.store(&maps.out[0], at_block, col, first_row);
       if (PARTS == 2) out.store(&maps.out[1], kOutBytes / 2, col, first_row);
       out.end();
     } else {
       if (col >= e.d || (t.job == 1 && first_row >= e.width)) return;
-      out.begin();
+      int at_block = 0;
       if (PARTS == 2 || t.job == 0) {
+        out.template begin<kOutBytes>();
 #pragma unroll
         for (int q = 0; q < 8; ++q)
-          out.put<128>(0, q, *reinterpret_cast<const uint4*>(v + 4 * q));
+          out.template put<128>(0, q, *reinterpret_cast<const uint4*>(v + 4 * q));
       } else {
+        at_block = out.template begin<kOutBytes / 2>();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) out.put<64>(0, q, pack_bf16(v + 8 * q));
+        for (int q = 0; q < 4; ++q) out.template put<64>(at_block, q, pack_bf16(v + 8 * q));
       }
       out.written();
-      if (t.job == 1) out.store(&maps.out[1], 0, col, e.v0 + first_row);
+      if (t.job == 1) out.store(&maps.out[1], at_block, col, e.v0 + first_row);
       else if (e.add) out.add(&maps.out[0], 0, col, t.split * (int)e.n_pad + first_row);
       else out.store(&maps.out[0], 0, col, t.split * (int)e.n_pad + first_row);
       out.end();
@@ -674,7 +737,17 @@ __device__ __forceinline__ bool load_stages(const Maps& maps, const Args& e, con
   return true;
 }
 
-// The products of one tile, kChunk stages per accumulator (float32) or all of them.
+// Stages of K per accumulator, 0: all. float32: 2 stages, 24 steps, of which each stage's 8 with the low parts come
+// first: a step truncates by half a unit of the sum so far on average, so it is the 4 of hi hi per stage that cost.
+// (4 stages with the parts interleaved: dh of 46 tokens 1.2e-6 off, plain float32 sums 0.4e-6.) Losses of bfloat16
+// logits: 16 stages, 64 steps (all 128 of a hidden size of 2048: losses 1.0e-6 off). bfloat16 gradients are rounded to
+// 2^-8 afterwards and need none.
+template <int PARTS, int EPI>
+__host__ __device__ constexpr int chunk_of() {
+  return PARTS == 2 ? 2 : EPI == kStats ? 16 : 0;
+}
+
+// The products of one tile.
 template <int PARTS, int EPI, int JOB>
 __device__ __forceinline__ bool multiply_stages(const Tile& t, uint32_t tmem_base, uint8_t* smem, uint64_t* full,
                                                 uint64_t* empty, uint64_t* tfull, uint64_t* tempty, Ring& ring, Ring& acc,
@@ -684,7 +757,8 @@ __device__ __forceinline__ bool multiply_stages(const Tile& t, uint32_t tmem_bas
   constexpr uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | ((uint32_t)M::kA << 15) |
                              ((uint32_t)M::kB << 16) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
   constexpr uint32_t a_step = M::kA ? 2048 : 32, b_step = M::kB ? 2048 : 32;   // bytes of 16 k
-  const int chunk = PARTS == 2 ? kChunk : t.last - t.first;
+  constexpr int kChunk = chunk_of<PARTS, EPI>();
+  const int chunk = kChunk > 0 ? kChunk : t.last - t.first;
   for (int first = t.first; first < t.last; first += chunk) {
     if (!warp_wait(&tempty[acc.at], acc.phase ^ 1, abort_flag)) return false;
     fence_after();
@@ -695,17 +769,18 @@ __device__ __forceinline__ bool multiply_stages(const Tile& t, uint32_t tmem_bas
       fence_after();
       if (elect_one()) {
         const uint32_t base = smem_u32(smem + ring.at * Stages<PARTS>::kBytes);
+        auto multiply = [&](uint32_t a, uint32_t b, bool fresh) {
 #pragma unroll
-        for (int k = 0; k < kBlockK / 16; ++k) {
-          const uint64_t a = operand_desc(base + a_step * k, M::kA);
-          const uint64_t b = operand_desc(base + kOperandBytes + b_step * k, M::kB);
-          mma_pair(d_tmem, a, b, idesc, kb != first || k != 0);
-          if constexpr (PARTS == 2) {
-            const uint64_t a_lo = operand_desc(base + 2 * kOperandBytes + a_step * k, M::kA);
-            const uint64_t b_lo = operand_desc(base + 3 * kOperandBytes + b_step * k, M::kB);
-            mma_pair(d_tmem, a, b_lo, idesc, 1);
-            mma_pair(d_tmem, a_lo, b, idesc, 1);
-          }
+          for (int k = 0; k < kBlockK / 16; ++k)
+            mma_pair(d_tmem, operand_desc(base + a * kOperandBytes + a_step * k, M::kA),
+                     operand_desc(base + b * kOperandBytes + b_step * k, M::kB), idesc, !fresh || kb != first || k != 0);
+        };
+        if constexpr (PARTS == 2) {
+          multiply(0, 3, true);      // hi lo
+          multiply(2, 1, false);     // lo hi
+          multiply(0, 1, false);
+        } else {
+          multiply(0, 1, true);
         }
         commit_pair(&empty[ring.at]);
         if (kb == last - 1) commit_pair(&tfull[acc.at]);
@@ -756,6 +831,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
   cluster_sync();
   fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  depend();
 
   const int kept = *e.s.kept;
   const Extent extent[2] = {extent_of(e.job[0], kept), extent_of(e.job[1], kept)};
@@ -813,39 +889,36 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
     const int quarter = warp & 3, half = (warp - 2) >> 2;
     const uint32_t lane_base = tmem_base + ((uint32_t)(quarter * 32) << 16) + half * 128;
     const int warp_row = (int)rank * 128 + quarter * 32;
-    const BlockOut block{smem + kStageBytes + (warp - 2) * kOutBytes, lane};
+    BlockOut block{smem + kStageBytes + (warp - 2) * kOutBytes, lane, 0, false};
     const uint32_t release[2] = {at_leader(&tempty[0]), at_leader(&tempty[1])};
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    constexpr int kChunk = chunk_of<PARTS, EPI>();
+    Ring acc;
     bool ok = true;
     for (int index = pair; index < tiles && ok; index += pairs) {
       const Tile t = tile_of<EPI>(index, extent, e);
       RowEpilogue<PARTS, EPI> out(maps, e, block, t, warp_row, kept);
       const int col = t.n * kTile + half * 128;
-      if constexpr (PARTS == 2) {
+      auto release_buffer = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(release[acc.at]);
+        acc.next(2);
+      };
+      if constexpr (kChunk > 0) {
         float total[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) total[j] = 0.f;
         for (int first = t.first; first < t.last; first += kChunk) {
-          if (!mbar_wait(&tfull[acc], acc_phase, abort_flag, kWaitNs)) {
-            ok = false;
-            break;
-          }
+          if (!(ok = warp_wait(&tfull[acc.at], acc.phase, abort_flag))) break;
           fence_after();
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float v[32];
-            tmem_ld32(lane_base + acc * kTile + 32 * c, v);
+            tmem_ld32(lane_base + acc.at * kTile + 32 * c, v);
 #pragma unroll
             for (int j = 0; j < 32; ++j) total[32 * c + j] += v[j];
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(release[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
+          release_buffer();
         }
         if (!ok) break;
 #pragma unroll
@@ -857,37 +930,26 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
         }
       } else {
         const bool any = t.first < t.last;
-        if (any && !mbar_wait(&tfull[acc], acc_phase, abort_flag, kWaitNs)) {
-          ok = false;
-          break;
-        }
+        if (any && !(ok = warp_wait(&tfull[acc.at], acc.phase, abort_flag))) break;
         fence_after();
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float v[32];
           if (any) {
-            tmem_ld32(lane_base + acc * kTile + 32 * c, v);
+            tmem_ld32(lane_base + acc.at * kTile + 32 * c, v);
           } else {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] = 0.f;
           }
           out.columns(v, col + 32 * c);
         }
-        if (any) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_at(release[acc]);
-          if (++acc == 2) {
-            acc = 0;
-            acc_phase ^= 1;
-          }
-        }
+        if (any) release_buffer();
       }
       out.finish(2 * t.n + half);
     }
     block.finish();
-    if (!ok) {
-      if (lane == 0) atomicCAS(&g_error, 0, kErrEpilogue);
+    if (!ok && lane == 0) {
+      atomicCAS(&g_error, 0, kErrEpilogue);
       *abort_flag = 1;
     }
   }
@@ -902,7 +964,6 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
 }
 
 // ---- per-row kernels ----------------------------------------------------------------------------------------------
-// lse and loss of the kept rows from the column parts' maxima and sums: 32 rows a block, its 32 warps sharing the parts.
 __device__ __forceinline__ void merge(float& top, float& sum, float top2, float sum2) {
   const float most = fmaxf(top, top2);
   if (most > -INFINITY) sum = sum * exp2f((top - most) * kLog2e) + sum2 * exp2f((top2 - most) * kLog2e);
@@ -910,20 +971,138 @@ __device__ __forceinline__ void merge(float& top, float& sum, float top2, float 
   top = most;
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------------------
+// The logits of up to ROWS kept float32 rows (the groups of blockIdx.y) reduced to statistics: bound by reading the head
+// once. A warp takes BATCH rows of the head at a time, 16 bytes a lane and row, against the hidden rows in shared
+// memory, then adds its BATCH x ROWS sums across its lanes by halving: lane l ends with the sum of index l / (32 / (BATCH
+// x ROWS)).
+template <int ROWS, int BATCH>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const float* hidden, int64_t stride, const float* head,
+                                                          const int64_t* targets, int64_t ignore, int n, int d, int vocab,
+                                                          float2* stats, int64_t n_pad, float* picked, float* losses,
+                                                          State s) {
+  constexpr int kSums = ROWS * BATCH;
+  static_assert(kSums <= 32 && (kSums & (kSums - 1)) == 0, "one sum a lane at most");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  float* rows = reinterpret_cast<float*>(smem_raw);                       // [ROWS][d]
+  __shared__ int row_of[32], target_of[32], kept_rows;
+  __shared__ float2 shared[kFewWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = blockIdx.y * ROWS;
+  depend();
+  if (warp == 0) {
+    const int64_t target = lane < n ? targets[lane] : ignore;
+    const bool keep = lane < n && is_kept(target, ignore, vocab);
+    const unsigned mask = __ballot_sync(0xffffffffu, keep);
+    const int at = __popc(mask & ((1u << lane) - 1u));
+    const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
+    if (keep) {
+      row_of[at] = lane;
+      target_of[at] = (int)target;
+      if (writes) {
+        s.row_of[at] = lane;
+        s.target[at] = (int)target;
+      }
+    }
+    if (writes && lane < n) {
+      s.place_of[lane] = keep ? at : -1;
+      if (!keep) losses[lane] = target == ignore ? 0.f : NAN;
+    }
+    if (lane == 0) {
+      kept_rows = __popc(mask);
+      if (writes) {
+        *s.kept = kept_rows;
+        *s.arrived = 0;
+      }
+    }
+  }
+  __syncthreads();
+  const int kept = kept_rows;
+  if (first >= kept) return;
+  for (int i = threadIdx.x; i < ROWS * d; i += kFewThreads) {
+    const int r = i / d, c = i % d;
+    const float v = first + r < kept ? hidden[row_of[first + r] * stride + c] : 0.f;
+    rows[i] = v;
+    if (blockIdx.x == 0 && first + r < kept) s.raw[(int64_t)first * d + i] = v;
+  }
+  __syncthreads();
+
+  constexpr int kCopies = 32 / kSums;                    // lanes that end with the same sum
+  const int index = lane / kCopies, row = index % ROWS, batch_row = index / ROWS;
+  const int target = first + row < kept ? target_of[first + row] : -1;
+  float top = -INFINITY, sum = 0.f;
+  const int step = gridDim.x * kFewWarps * BATCH;
+  for (int v0 = (blockIdx.x * kFewWarps + warp) * BATCH; v0 < vocab; v0 += step) {
+    float acc[kSums] = {};
+#pragma unroll 2
+    for (int c = lane * 4; c < d; c += 128) {
+      float4 w[BATCH];
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b)
+        w[b] = __ldcs(reinterpret_cast<const float4*>(head + (int64_t)min(v0 + b, vocab - 1) * d + c));
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float4 h = *reinterpret_cast<const float4*>(rows + r * d + c);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+          float& a = acc[b * ROWS + r];
+          a = fmaf(h.x, w[b].x, a);
+          a = fmaf(h.y, w[b].y, a);
+          a = fmaf(h.z, w[b].z, a);
+          a = fmaf(h.w, w[b].w, a);
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16, count = kSums; o > 0; o >>= 1) {
+      if (count > 1) {
+        count /= 2;
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < kSums / 2; ++i)
+          if (i < count) {
+            const float own = upper ? acc[i + count] : acc[i], sent = upper ? acc[i] : acc[i + count];
+            acc[i] = own + __shfl_xor_sync(0xffffffffu, sent, o);
+          }
+      } else {
+        acc[0] += __shfl_xor_sync(0xffffffffu, acc[0], o);
+      }
+    }
+    const int v = v0 + batch_row;
+    if (v < vocab) {
+      const float z = acc[0];
+      if (v == target) picked[first + row] = z;
+      merge(top, sum, z, 1.f);
+    }
+  }
+  shared[warp][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (threadIdx.x < ROWS && first + threadIdx.x < kept) {
+    top = -INFINITY;
+    sum = 0.f;
+    for (int w = 0; w < kFewWarps; ++w)
+      for (int b = 0; b < BATCH; ++b) {
+        const float2 part = shared[w][(b * ROWS + threadIdx.x) * kCopies];
+        merge(top, sum, part.x, part.y);
+      }
+    stats[blockIdx.x * n_pad + first + threadIdx.x] = make_float2(top, sum);
+  }
+}
+
+// ---- losses -------------------------------------------------------------------------------------------------------
+// lse and loss of the kept rows from the parts' maxima and sums: 32 rows a block, its 32 warps sharing the parts.
 // The block that finishes last also adds up the losses where their sum or mean is asked for (float64, the same order
-// whichever block that is). The blocks after the `row_blocks` zero the kept rows up to a whole stage of K of the dw
-// product.
+// whichever block that is). The blocks after the `row_blocks` (bfloat16) zero the kept rows up to a whole stage of K of
+// the dw product.
 __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* stats, int64_t n_pad, int parts,
                                                       const float* picked, float* losses, int n, int reduction,
-                                                      float* loss, int row_blocks, int row_bytes, int operands) {
+                                                      float* loss, int row_blocks, int row_bytes) {
   __shared__ float2 shared[32][33];
+  depend();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane, kept = *s.kept;
   if (blockIdx.x >= row_blocks) {
     const int64_t step = (int64_t)(gridDim.x - row_blocks) * 1024, end = round_up(kept, kBlockK) * row_bytes / 16;
-    for (int part = 0; part < operands; ++part)
-      for (int64_t i = (int64_t)kept * row_bytes / 16 + (blockIdx.x - row_blocks) * 1024 + threadIdx.x; i < end;
-           i += step)
-        static_cast<uint4*>(s.hidden[part])[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = (int64_t)kept * row_bytes / 16 + (blockIdx.x - row_blocks) * 1024 + threadIdx.x; i < end; i += step)
+      static_cast<uint4*>(s.hidden[0])[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   if (blockIdx.x * 32 < kept) {
@@ -979,6 +1158,7 @@ __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* sta
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(State s, const float* slots, int splits, int64_t n_pad,
                                                       Upstream upstream, T* grad_hidden, int n, int d) {
+  depend();
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t >= n) return;
   const int at = s.place_of[t];
@@ -1066,22 +1246,46 @@ static int operand_map(CUtensorMap* map, int dtype, const void* base, int64_t ro
   return make_map(map, part_type(dtype), base, rows, columns, ld, kBlockK, box_rows);
 }
 
-template <int PARTS, int EPI>
-static int launch_products(const Maps& maps, const Args& e, int64_t most_tiles, cudaStream_t st) {
-  auto kernel = product_kernel<PARTS, EPI>;
-  static bool configured[kMaxDevices] = {};
-  int device = 0;
+// Raises a kernel's limit of dynamic shared memory, once per device.
+template <auto kernel>
+static int allow_shared_memory(int bytes) {
+  static bool done[kMaxDevices] = {};
+  int device = -1;
   cudaGetDevice(&device);
-  if (device < 0 || device >= kMaxDevices || !configured[device]) {
-    const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (r != cudaSuccess) {
-      set_error("linear_ce: %s", cudaGetErrorString(r));
-      return HFFN_ERR_CUDA;
-    }
-    if (device >= 0 && device < kMaxDevices) configured[device] = true;
+  const bool known = device >= 0 && device < kMaxDevices;
+  if (known && done[device]) return HFFN_OK;
+  const cudaError_t r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (r != cudaSuccess) {
+    set_error("linear_ce: %s", cudaGetErrorString(r));
+    return HFFN_ERR_CUDA;
   }
+  if (known) done[device] = true;
+  return HFFN_OK;
+}
+
+// Launches a kernel that may start while the kernel before it in the stream, one of the same call, still runs.
+template <auto kernel, typename... A>
+static void launch_next(unsigned grid, unsigned threads, size_t shared, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = shared;
+  config.stream = st;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, kernel, args...);     // its error is the next launch_status'
+}
+
+// next: the kernel before it in the stream is one of the same call.
+template <int PARTS, int EPI>
+static int launch_products(const Maps& maps, const Args& e, int64_t most_tiles, bool next, cudaStream_t st) {
+  HFFN_TRY((allow_shared_memory<product_kernel<PARTS, EPI>>(kSmem)));
   const int pairs = (int)std::min<int64_t>(sm_pairs(), most_tiles);
-  kernel<<<2 * pairs, kThreads, kSmem, st>>>(maps, e);
+  if (next) launch_next<product_kernel<PARTS, EPI>>(2 * pairs, kThreads, kSmem, st, maps, e);
+  else product_kernel<PARTS, EPI><<<2 * pairs, kThreads, kSmem, st>>>(maps, e);
   return launch_status("linear_ce product");
 }
 
@@ -1098,6 +1302,18 @@ static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_
   return HFFN_OK;
 }
 
+constexpr int kFewBlocks = 148 * 3;    // of the few-row kernel: 24 warps an SM
+
+template <int ROWS, int BATCH>
+static int launch_few(const float* hidden, int64_t stride, const float* head, const int64_t* targets, int64_t ignore,
+                      int n, int d, int vocab, float2* stats, int64_t n_pad, float* picked, float* losses, const State& s,
+                      int blocks, cudaStream_t st) {
+  HFFN_TRY((allow_shared_memory<few_kernel<ROWS, BATCH>>((int)kFewBytes)));
+  few_kernel<ROWS, BATCH><<<dim3(blocks, (unsigned)ceil_div(n, ROWS)), kFewThreads, ROWS * d * 4, st>>>(
+      hidden, stride, head, targets, ignore, n, d, vocab, stats, n_pad, picked, losses, s);
+  return launch_status("linear_ce few rows");
+}
+
 struct ForwardWork {
   float2* stats;
   float *picked, *losses;
@@ -1108,7 +1324,7 @@ static ForwardWork forward_work(void* base, int64_t n, int vocab) {
   Carve c{static_cast<uint8_t*>(base)};
   const int64_t n_pad = round_up(n, kTile);
   ForwardWork w;
-  w.stats = c.take<float2>(2 * ceil_div(vocab, kTile) * n_pad);
+  w.stats = c.take<float2>(std::max<int64_t>(2 * ceil_div(vocab, kTile), kFewBlocks) * n_pad);
   w.picked = c.take<float>(n_pad);
   w.losses = c.take<float>(n_pad);
   w.bytes = c.at;
@@ -1146,6 +1362,10 @@ static int check(int dtype, int64_t n, int32_t d, int32_t vocab) {
   return HFFN_OK;
 }
 
+static int measuring_blocks(int vocab, int d) {
+  return (int)std::min<int64_t>(148 * 8, ceil_div((int64_t)vocab * d, 4 * kGatherThreads));
+}
+
 template <typename T>
 static int forward(const void* hidden, int64_t stride, const void* weight, const int64_t* targets, int64_t ignore,
                    int reduction, float* loss, void* state, void* work, int n, int d, int vocab, cudaStream_t st) {
@@ -1160,22 +1380,36 @@ static int forward(const void* hidden, int64_t stride, const void* weight, const
   e.stats = w.stats;
   e.picked = w.picked;
   float* losses = reduction == HFFN_REDUCE_NONE ? loss : w.losses;
-  const int span = (int)std::max<int64_t>(16, ceil_div(n, 512)), gather = (int)ceil_div(n, span);
-  const bool aligned = (reinterpret_cast<uintptr_t>(hidden) & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
-  if (PARTS == 2 && cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
-  const int measure = PARTS == 2 ? (int)std::min<int64_t>(148 * 8, ceil_div((int64_t)vocab * d, 4 * kGatherThreads)) : 0;
-  gather_kernel<T><<<gather + measure, kGatherThreads, 0, st>>>(static_cast<const T*>(hidden), stride,
-                                                                static_cast<const T*>(weight), targets, ignore, n, d,
-                                                                vocab, span, gather, aligned, losses, e.s);
-  if constexpr (PARTS == 2)
-    split_kernel<<<(unsigned)ceil_div((int64_t)vocab + n, 8), 256, 0, st>>>(
-        static_cast<const float*>(hidden), stride, aligned, static_cast<const float*>(weight), d, vocab, e.s);
-  Maps maps;
-  HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
-  HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), st)));
+  const T *rows = static_cast<const T*>(hidden), *head = static_cast<const T*>(weight);
+  int parts = 0;
+  if (is_few(dtype, n, d)) {
+    if constexpr (PARTS == 2) {
+      parts = (int)std::min<int64_t>(kFewBlocks, ceil_div(vocab, kFewWarps * 4));
+      const int each = few_rows(n);
+      auto few = each == 1   ? launch_few<1, 8>
+                 : each == 2 ? launch_few<2, 8>
+                 : each == 4 ? launch_few<4, 4>
+                             : launch_few<kFewRows, 4>;
+      HFFN_TRY(few(rows, stride, head, targets, ignore, n, d, vocab, w.stats, e.n_pad, w.picked, losses, e.s, parts, st));
+    }
+  } else {
+    const int span = (int)std::max<int64_t>(16, ceil_div(n, 512)), gather = (int)ceil_div(n, span);
+    const bool aligned = (reinterpret_cast<uintptr_t>(hidden) & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
+    if (PARTS == 2 && cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
+    const int measure = PARTS == 2 ? measuring_blocks(vocab, d) : 0;
+    gather_kernel<T><<<gather + measure, kGatherThreads, 0, st>>>(rows, stride, head, targets, ignore, n, d, vocab, span,
+                                                                  gather, aligned, losses, e.s);
+    if constexpr (PARTS == 2)
+      launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, rows, stride, aligned,
+                                head, d, vocab, e.s);
+    Maps maps;
+    HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
+    HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), true, st)));
+    parts = 2 * (int)ceil_div(vocab, kTile);
+  }
   const int row_blocks = (int)ceil_div(n, 32);
-  losses_kernel<<<row_blocks + 4, 1024, 0, st>>>(e.s, w.stats, e.n_pad, 2 * (int)ceil_div(vocab, kTile), w.picked, losses,
-                                                 n, reduction, loss, row_blocks, 2 * d, PARTS);
+  launch_next<losses_kernel>(row_blocks + (PARTS == 1 ? 4 : 0), 1024, 0, st, e.s, w.stats, e.n_pad, parts, w.picked,
+                             losses, n, reduction, loss, row_blocks, 2 * d);
   return launch_status("linear_ce_forward");
 }
 
@@ -1192,6 +1426,17 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
   e.vocab = vocab;
   e.n_pad = round_up(n, kTile);
   e.upstream = {grad_loss, reduction};
+  bool prepared = false;             // a kernel of this call precedes the products
+  if constexpr (PARTS == 2) {
+    if (is_few(dtype, n, d)) {       // the forward has made no parts
+      const float* values = static_cast<const float*>(weight);
+      if (cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
+      measure_kernel<<<1 + measuring_blocks(vocab, d), kGatherThreads, 0, st>>>(values, d, vocab, e.s);
+      launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, (const float*)nullptr,
+                                (int64_t)0, true, values, d, vocab, e.s);
+      prepared = true;
+    }
+  }
   const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
   if (PARTS == 2) {
     e.dw_rows_largest = e.s.largest;
@@ -1205,7 +1450,8 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
       const unsigned blocks = (unsigned)(e.n_pad / 8);
       scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
-      scaled_rows_kernel<true><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
+      launch_next<scaled_rows_kernel<true>>(blocks, 256, 0, st, e.s, e.upstream, w.largest, hi, lo, d);
+      prepared = true;
     }
   }
   const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
@@ -1219,7 +1465,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
     HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
     for (int part = 0; part < PARTS; ++part)
       HFFN_TRY(make_map(&maps.out[part], part_type(dtype), w.g[part], e.n_pad, width, width, 32, 32));
-    HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, st)));
+    HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, v0 > 0 || prepared, st)));
     e.jobs = 0;
     int64_t tiles = 0;
     if (grad_hidden != nullptr) {
@@ -1245,11 +1491,11 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       e.jobs = 2;
       tiles += columns * wide;
     }
-    if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, st)));
+    if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, true, st)));
   }
   if (grad_hidden != nullptr)
-    scatter_kernel<T><<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(e.s, w.slots, splits, e.n_pad, e.upstream,
-                                                                static_cast<T*>(grad_hidden), n, d);
+    launch_next<scatter_kernel<T>>((unsigned)ceil_div(n, 8), 256, 0, st, e.s, (const float*)w.slots, splits, e.n_pad,
+                                   e.upstream, static_cast<T*>(grad_hidden), n, d);
   return launch_status("linear_ce_backward");
 }
 

@@ -72,7 +72,7 @@ def grad_norm(tensors) -> torch.Tensor:
     with native.on_device(tensors.device):
         native.check(native.lib.hffn_grad_norm(len(tensors), _address(tensors.pointers), _address(tensors.counts),
                                                _address(tensors.types), norm.data_ptr(), work.data_ptr(),
-                                               native.stream_handle(tensors.device)), "hffn_grad_norm")
+                                               native.raw_stream(tensors.device)), "hffn_grad_norm")
     return norm
 
 
@@ -102,6 +102,6 @@ def clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
         native.check(native.lib.hffn_clip_grad_norm(
             len(tensors), _address(tensors.pointers), _address(outs.pointers), _address(tensors.counts),
             _address(tensors.types), _address(outs.types), float(max_norm), norm.data_ptr(), work.data_ptr(),
-            native.stream_handle(tensors.device)), "hffn_clip_grad_norm")
+            native.raw_stream(tensors.device)), "hffn_clip_grad_norm")
     torch.autograd.graph.increment_version(outs.tensors)
     return norm

@@ -60,7 +60,7 @@ def _forward(hidden, weight, targets, ignore_index, reduction):
         native.check(native.lib.hffn_linear_ce_forward(
             code, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), targets.data_ptr(), ignore_index,
             native.REDUCE_CODES[reduction], loss.data_ptr(), state.data_ptr(), work.data_ptr(), n, d, vocab,
-            native.stream_handle(device)), "hffn_linear_ce_forward")
+            native.raw_stream(device.index)), "hffn_linear_ce_forward")
     return loss, state
 
 
@@ -74,7 +74,7 @@ def _backward(weight, state, n, reduction, grad_loss, want_hidden=True, want_wei
         native.check(native.lib.hffn_linear_ce_backward(
             code, weight.data_ptr(), native.REDUCE_CODES[reduction], grad_loss.data_ptr(),
             grad_hidden.data_ptr() if want_hidden else None, grad_weight.data_ptr() if want_weight else None,
-            state.data_ptr(), work.data_ptr(), n, d, vocab, native.stream_handle(device)), "hffn_linear_ce_backward")
+            state.data_ptr(), work.data_ptr(), n, d, vocab, native.raw_stream(device.index)), "hffn_linear_ce_backward")
     return grad_hidden, grad_weight
 
 

@@ -131,6 +131,13 @@ def test_against_float64(n, d, v, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9, 17, 32, 33])
+@pytest.mark.parametrize("d,v", [(8, 3), (520, 1027), (2048, 700), (4096, 300)])
+def test_few_rows(n, d, v, dtype):
+    check(*make(n, d, v, dtype, seed=n + d, ignored=0.2))
+
+
+@BOTH
 @pytest.mark.parametrize("reduction", ["mean", "sum"])
 @pytest.mark.parametrize("ignored", [0.0, 0.3])
 def test_reductions(reduction, ignored, dtype):
@@ -262,8 +269,8 @@ def test_shapes_and_strides(dtype):
     assert torch.equal(shifted.reshape(-1), same)
     one = linear_cross_entropy(h[3], w, t[3], reduction="none")                                      # a single token
     assert one.shape == () and abs(float(one - plain[3])) <= 1e-5 * float(plain[3])
-    repeated = h[:1].expand(5, 64)
-    assert torch.equal(linear_cross_entropy(repeated, w, t[:1].expand(5), reduction="none"), plain[:1].expand(5))
+    repeated = linear_cross_entropy(h[:1].expand(5, 64), w, t[:1].expand(5), reduction="none")       # no stride
+    assert torch.equal(repeated, linear_cross_entropy(h[:1].repeat(5, 1), w, t[:1].repeat(5), reduction="none"))
 
 
 @BOTH
