@@ -9,6 +9,8 @@ _LAZY = {
     "HFFNLayer": "runtime", "HFFNRuntime": "runtime", "UP_MODES": "runtime", "DOWN_MODES": "runtime",
     "MAX_TOKENS": "runtime", "up_mode": "runtime", "down_mode": "runtime",
     "HFFNTrainRuntime": "train_runtime", "transposed_supports": "train_runtime",
+    "linear_cross_entropy": "losses", "linear_cross_entropy_gradients": "losses",
+    "grad_norm": "grad_clip", "clip_grad_norm": "grad_clip",
 }
 
 

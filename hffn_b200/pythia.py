@@ -217,6 +217,43 @@ def load_pythia(model_dir: str | Path, export_dir: str | Path, ffn: str, device:
     return model
 
 
+def causal_lm_loss(model: nn.Module, input_ids: torch.Tensor, labels: torch.Tensor | None = None,
+                   ignore_index: int = -100, reduction: str = "mean", **inputs) -> torch.Tensor:
+    """The next-token loss of a Pythia model (any arm) without its logits: ``losses.linear_cross_entropy`` of the last
+    hidden states under ``embed_out``, position t against ``labels[:, t + 1]`` (``labels`` [batch, length], default
+    ``input_ids``; ``ignore_index`` where a token is not trained on). ``reduction="none"``: the losses [batch, length],
+    0 in the last position, which predicts nothing. ``inputs``: further inputs of the model (``attention_mask``, ...).
+    Differentiable for a trainable model; scoring under ``torch.no_grad()`` for any."""
+    from .losses import linear_cross_entropy
+    labels = input_ids if labels is None else labels
+    if labels.shape != input_ids.shape or labels.dim() != 2:
+        raise ValueError("expected input_ids and labels [batch, length]")
+    targets = torch.full_like(labels, ignore_index)
+    targets[:, :-1] = labels[:, 1:]
+    hidden = model.gpt_neox(input_ids=input_ids, **inputs).last_hidden_state
+    return linear_cross_entropy(hidden, model.embed_out.weight, targets, ignore_index, reduction)
+
+
+def train_step(model: nn.Module, optimizer, input_ids: torch.Tensor, labels: torch.Tensor | None = None,
+               max_norm: float | None = None, **inputs) -> tuple[torch.Tensor, torch.Tensor]:
+    """One training step of a ``load_pythia(..., trainable=True)`` model: ``causal_lm_loss``, backward, the gradients of
+    the FFNs and of every other parameter clipped together to ``max_norm`` (None: their norm only), ``optimizer`` (over
+    the model's other parameters) and the FFNs' compact AdamW. Returns the loss of the parameters before the update and
+    the gradients' norm before clipping, both scalars on the device; the host waits for nothing."""
+    train = getattr(model, "hffn_train", None)
+    if train is None:
+        raise ValueError("train_step needs a model loaded with trainable=True")
+    optimizer.zero_grad(set_to_none=True)
+    loss = causal_lm_loss(model, input_ids, labels, **inputs)
+    loss.backward()
+    others = [p.grad for p in model.parameters() if p.grad is not None]
+    norm = train.clip_grad_norm(float("inf") if max_norm is None else max_norm, others)
+    optimizer.step()
+    for index in range(len(train.steps)):
+        train.adamw(index)
+    return loss.detach(), norm
+
+
 def _world(group) -> int:
     import torch.distributed as dist
     return dist.get_world_size(group)

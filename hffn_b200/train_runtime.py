@@ -323,6 +323,17 @@ class HFFNTrainRuntime:
         """AdamW from the stored gradients (after a data-parallel exchange); the dense operands are rebuilt lazily."""
         self.adamw(index)
 
+    def clip_grad_norm(self, max_norm: float, tensors=(), layers=None) -> torch.Tensor:
+        """Clip the stored compact gradients of ``layers`` (indices; default all) together with ``tensors`` (the
+        gradients of a model's other parameters) by their global norm, in place, before ``adamw``: every entry times
+        ``min(1, max_norm / (norm + 1e-6))``. Returns the norm before it, a float32 scalar on the device
+        (``grad_clip.clip_grad_norm``; no host synchronisation). The steps that fuse AdamW into the backward (``step``,
+        ``step_mse``) apply their gradients unclipped."""
+        from .grad_clip import clip_grad_norm
+        layers = range(len(self._grads)) if layers is None else layers
+        compact = [grad for index in layers for grad in self._grads[index].values()]
+        return clip_grad_norm([*compact, *tensors], max_norm)
+
     # -- stacks of layers: every call keeps its own activations ---------------------------------------------------
     def forward_saved(self, index: int, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """``(y, z, act)`` of layer ``index`` for x[N, d_model], each a new tensor (z and act hidden-major
