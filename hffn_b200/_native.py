@@ -106,8 +106,8 @@ SIGNATURES = {
     "hffn_forward_noalloc": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(Layer), _P, _P, _I64, _P]),
     "hffn_linear_ce_state_bytes": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
     "hffn_linear_ce_forward_workspace": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
-    "hffn_linear_ce_forward": (ctypes.c_int, [ctypes.c_int, _P, _I64, _P, _P, _I64, ctypes.c_int, _P, _P, _P, _I64,
-                                              _I32, _I32, _P]),
+    "hffn_linear_ce_forward": (ctypes.c_int, [ctypes.c_int, _P, _I64, _P, _P, _I64, ctypes.c_int, ctypes.c_int, _P, _P,
+                                              _P, _I64, _I32, _I32, _P]),
     "hffn_linear_ce_backward_workspace": (_I64, [ctypes.c_int, _I64, _I32, _I32]),
     "hffn_linear_ce_backward": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_int, _P, _P, _P, _P, _P, _I64, _I32, _I32,
                                                _P]),

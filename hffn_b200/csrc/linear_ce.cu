@@ -21,7 +21,9 @@
 // 2^e one power of two per operand that brings its largest finite entry to [2^14, 2^15): entries down to 2^-17 of the
 // largest keep 22 bits, smaller ones are held to 2^-39 of it. One scale per operand, not per row, because each of h, w
 // and g is summed over its rows in one of the products. g holds 2^14 (p - [v = target]), c_t is applied in float32
-// afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). Sums: the
+// afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). A forward
+// without a backward takes a scale for each row of the head instead, which saves the pass that finds the largest entry
+// (2048 x 1024 x 50304: 50 of 600 us). Sums: the
 // tensor core's float32 accumulation truncates at every step, so what ends in float32 (float32 gradients, losses) is
 // summed in registers from accumulators of few steps each (chunk_of).
 #include <cuda_fp16.h>
@@ -62,9 +64,10 @@ struct State {
   int32_t* row_of;     // [n] the input row of each kept row
   int32_t* place_of;   // [n] the kept row of each input row; -1: left out
   int32_t* target;     // [n]
-  float* lse;          // [n]
+  float2* sums;        // [n] of each kept row the largest logit and the sum of exponentials relative to it
   void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts)
   void* head[2];       // [vocab, d] float32: the head's fp16 parts
+  float* inverse;      // [vocab] float32, no backward: the inverse scale of each row of the head
   float* raw;          // [kFew, d] float32, few rows: the kept rows as they are (their parts are made in the backward)
   int64_t bytes;
 };
@@ -80,19 +83,21 @@ struct Carve {
   }
 };
 
-// Few float32 rows: their logits are computed on the CUDA cores, straight from the head (few_kernel), where that is
-// faster than making the head's fp16 parts for the tensor cores (two passes over it and one of writes before the
-// products): d 1024, vocabulary 50304, whole calls: 50, 79 and 122 us for 1, 8 and 16 rows against 177; 32 rows would
-// take 228. (bfloat16 has no such detour: 38 us on the tensor cores for 1 to 32 rows, 34 with this kernel for one, 42 for
-// two.) The rows have to fit the kernel's shared memory.
+// Few rows: their logits are computed on the CUDA cores, straight from the head (few_kernel), where that is faster than
+// the tensor cores' tiles. float32: up to 16 rows, in passes of 8, since it spares making the head's fp16 parts (a pass
+// of reads and one of writes before the products): d 1024, vocabulary 50304, whole calls: 47, 82 and 125 us for 4, 8 and
+// 16 rows against 149; 32 rows would take 228. bfloat16: one row (31 us against 36; two rows 42). The rows have to fit
+// the kernel's shared memory.
 constexpr int kFewRows = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int64_t kFewBytes = 96 << 10;
 
 // Rows of one pass.
-static int few_rows(int64_t n) { return n <= 2 ? (int)n : n <= 4 ? 4 : kFewRows; }
+static int few_rows(int dtype, int64_t n) {
+  return dtype == HFFN_BF16 ? 1 : n <= kFewRows / 2 ? kFewRows / 2 : kFewRows;
+}
 
 static bool is_few(int dtype, int64_t n, int d) {
-  return dtype == HFFN_F32 && n <= 2 * kFewRows && (int64_t)few_rows(n) * d * 4 <= kFewBytes;
+  return n <= (dtype == HFFN_F32 ? 2 * kFewRows : 1) && (int64_t)few_rows(dtype, n) * d * 4 <= kFewBytes;
 }
 
 static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
@@ -105,11 +110,12 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   s.row_of = c.take<int32_t>(n_pad);
   s.place_of = c.take<int32_t>(n_pad);
   s.target = c.take<int32_t>(n_pad);
-  s.lse = c.take<float>(n_pad);
+  s.sums = c.take<float2>(n_pad);
   for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
   if (dtype == HFFN_F32)
     for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
-  if (is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
+  if (dtype == HFFN_F32) s.inverse = c.take<float>(vocab);
+  if (dtype == HFFN_F32 && is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
   s.bytes = c.at;
   return s;
 }
@@ -269,21 +275,34 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
 }
 
 // float32: the fp16 parts of the head and of the kept rows (from `hidden`, or from the state where `hidden` is NULL),
-// one warp a row; the kept rows are padded with zeros to a whole stage of K of the dw product.
+// one warp a row; the kept rows are padded with zeros to a whole stage of K of the dw product. by_row: each row of the
+// head at a scale of its own.
 __global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t stride, bool aligned, const float* head,
-                                                    int d, int vocab, State s) {
+                                                    int d, int vocab, bool by_row, State s) {
   depend();
   const int lane = threadIdx.x & 31, kept = *s.kept;
   int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   const bool of_head = row < vocab;
   if (!of_head) row -= vocab;
   if (!of_head && row >= (int)round_up(kept, kBlockK)) return;
-  const float scale = power_of_two(scale_exponent(s.largest[of_head]));
   const bool zero = !of_head && row >= kept;
   const float* from = of_head          ? head + (int64_t)row * d
                       : zero           ? nullptr
                       : hidden != NULL ? hidden + (int64_t)s.row_of[row] * stride
                                        : s.raw + (int64_t)row * d;
+  uint32_t bits = 0;
+  if (of_head && by_row) {
+#pragma unroll 4
+    for (int i = 4 * lane; i < d; i += 128) {
+      const float4 x = *reinterpret_cast<const float4*>(from + i);
+      bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
+    }
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    if (lane == 0) s.inverse[row] = power_of_two(-scale_exponent(bits));
+  } else {
+    bits = s.largest[of_head];
+  }
+  const float scale = power_of_two(scale_exponent(bits));
   __half* hi = static_cast<__half*>(of_head ? s.head[0] : s.hidden[0]) + (int64_t)row * d;
   __half* lo = static_cast<__half*>(of_head ? s.head[1] : s.hidden[1]) + (int64_t)row * d;
   for (int i = 8 * lane; i < d; i += 256) {
@@ -371,6 +390,7 @@ struct Args {
   float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials
   float* picked;           // kStats: [n_pad] the target's logit
   Upstream upstream;
+  const float* head_inverse;   // kStats, float32: of each row of the head (NULL: one scale for all)
   int add;                 // kGradients: dh adds to its slots (a later piece)
   const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
   int dw_upstream;                   // float32: dw's rows lack their c, which is the same for all
@@ -558,7 +578,8 @@ struct RowEpilogue {
   int target;
   float factor;             // of the accumulators
   float top, sum;           // kStats
-  float lse2, c;            // kGrad
+  float2 sums;              // kGrad
+  float lse2, c;
 
   __device__ __forceinline__ RowEpilogue(const Maps& maps_, const Args& args, BlockOut& out_, const Tile& tile,
                                          int warp_row, int kept)
@@ -574,11 +595,15 @@ struct RowEpilogue {
     } else {
       live = row < kept;
       target = live ? e.s.target[row] : -1;
-      if (PARTS == 2) factor = power_of_two(-scale_exponent(e.s.largest[0]) - scale_exponent(e.s.largest[1]));
+      if (PARTS == 2)
+        factor = power_of_two(-scale_exponent(e.s.largest[0]) -
+                              (EPI == kStats && e.head_inverse ? 0 : scale_exponent(e.s.largest[1])));
       top = -INFINITY;
       sum = 0.f;
       if (EPI == kGrad) {
-        lse2 = live ? e.s.lse[row] * kLog2e : 0.f;
+        sums = live ? e.s.sums[row] : make_float2(0.f, 1.f);
+        lse2 = (sums.x + logf(sums.y)) * kLog2e;
+        sums.y = 1.f / sums.y;
         c = PARTS == 2 ? 16384.f : live ? e.upstream.of(e.s, row, kept) : 0.f;
       }
     }
@@ -590,6 +615,19 @@ struct RowEpilogue {
       for (int j = 0; j < 32; ++j) v[j] *= factor;
     }
     if constexpr (EPI == kStats) {
+      if (PARTS == 2 && e.head_inverse) {
+        if (col + 32 <= e.vocab) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 x = __ldg(reinterpret_cast<const float4*>(e.head_inverse + col + j));
+            v[j] *= x.x, v[j + 1] *= x.y, v[j + 2] *= x.z, v[j + 3] *= x.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col + j < e.vocab) v[j] *= __ldg(e.head_inverse + col + j);
+        }
+      }
       if (col + 32 > e.vocab) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -604,17 +642,24 @@ struct RowEpilogue {
       float most = top;
 #pragma unroll
       for (int j = 0; j < 32; ++j) most = fmaxf(most, v[j]);
-      // a row of -inf so far has nothing to rescale; NaN logits reach the sum through their exponentials
-      const float base = most == -INFINITY ? 0.f : most * kLog2e;
-      float part[4] = {sum * exp2_fast(top * kLog2e - base), 0.f, 0.f, 0.f};
+      // a row of -inf so far has nothing to rescale; NaN logits reach the sum through their exponentials. The rounding
+      // of `base` (1e-6 of a logit of 16) is the same in all 32 exponents: it is taken out of their sum.
+      const bool none = most == -INFINITY;
+      const float base = none ? 0.f : most * kLog2e;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < 32; ++j) part[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -base));
-      sum = (part[0] + part[1]) + (part[2] + part[3]);
+      const float more = (part[0] + part[1]) + (part[2] + part[3]);
+      sum = none ? sum + more
+                 : fmaf(sum, exp2_fast((top - most) * kLog2e), more * exp2_fast(-fmaf(most, kLog2e, -base)));
       top = most;
     } else if constexpr (EPI == kGrad) {
       const int at = target - e.v0 - col;
+      // float32: relative to the largest logit, whose difference is exact where p is large (an argument rounded at
+      // the size of the logit puts 1e-6 on p, and p - 1 may be small)
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -lse2));
+      for (int j = 0; j < 32; ++j)
+        v[j] = PARTS == 2 ? exp2_fast((v[j] - sums.x) * kLog2e) * sums.y : exp2_fast(fmaf(v[j], kLog2e, -lse2));
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -739,28 +784,30 @@ __device__ __forceinline__ bool load_stages(const Maps& maps, const Args& e, con
   return true;
 }
 
-// Stages of K per accumulator, 0: all. float32: 2 stages, 24 steps, of which each stage's 8 with the low parts come
-// first: a step truncates by half a unit of the sum so far on average, so it is the 4 of hi hi per stage that cost.
-// (4 stages with the parts interleaved: dh of 46 tokens 1.2e-6 off, plain float32 sums 0.4e-6.) Losses of bfloat16
-// logits: 16 stages, 64 steps (all 128 of a hidden size of 2048: losses 1.0e-6 off). bfloat16 gradients are rounded to
-// 2^-8 afterwards and need none.
+// Stages of K per accumulator, 0: all. A step of 16 values truncates by half a unit of the sum so far on average.
+// float32: 2 stages, 24 steps, of which each stage's 8 with the low parts come first, so that it is the 4 of hi hi per
+// stage that cost (4 stages with the parts interleaved: dh of 46 tokens 1.2e-6 off, plain float32 sums 0.4e-6). Losses of
+// bfloat16 logits: 8 stages, 32 steps (8 x 511 tokens of 1024: 2.5e-7 off, plain sums 2.3e-7; 16 stages 5.2e-7 and no
+// faster; 4 stages 1.2e-7 but 8 to 15 % slower), and 4 where one row tile leaves the time to reading the head (few
+// losses average less, and that of a well predicted token is a small difference of logits). bfloat16 gradients are
+// rounded to 2^-8 afterwards and need none.
 template <int PARTS, int EPI>
-__host__ __device__ constexpr int chunk_of() {
-  return PARTS == 2 ? 2 : EPI == kStats ? 16 : 0;
+__device__ __forceinline__ int chunk_of(int kept) {
+  return PARTS == 2 ? 2 : EPI == kStats ? (kept <= kTile ? 4 : 8) : 0;
 }
 
 // The products of one tile.
 template <int PARTS, int EPI, int JOB>
-__device__ __forceinline__ bool multiply_stages(const Tile& t, uint32_t tmem_base, uint8_t* smem, uint64_t* full,
-                                                uint64_t* empty, uint64_t* tfull, uint64_t* tempty, Ring& ring, Ring& acc,
-                                                volatile int* abort_flag) {
+__device__ __forceinline__ bool multiply_stages(const Tile& t, int kept, uint32_t tmem_base, uint8_t* smem,
+                                                uint64_t* full, uint64_t* empty, uint64_t* tfull, uint64_t* tempty,
+                                                Ring& ring, Ring& acc, volatile int* abort_flag) {
   using M = Major<EPI, JOB>;
   constexpr uint32_t format = PARTS == 2 ? 0 : 1;   // fp16, bfloat16
   constexpr uint32_t idesc = (1u << 4) | (format << 7) | (format << 10) | ((uint32_t)M::kA << 15) |
                              ((uint32_t)M::kB << 16) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
   constexpr uint32_t a_step = M::kA ? 2048 : 32, b_step = M::kB ? 2048 : 32;   // bytes of 16 k
-  constexpr int kChunk = chunk_of<PARTS, EPI>();
-  const int chunk = kChunk > 0 ? kChunk : t.last - t.first;
+  int chunk = chunk_of<PARTS, EPI>(kept);
+  if (chunk == 0) chunk = t.last - t.first;
   for (int first = t.first; first < t.last; first += chunk) {
     if (!warp_wait(&tempty[acc.at], acc.phase ^ 1, abort_flag)) return false;
     fence_after();
@@ -867,9 +914,11 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
       for (int index = pair; index < tiles && ok; index += pairs) {
         const Tile t = tile_of<EPI>(index, extent, e);
         if (EPI == kGradients && t.job == 1)
-          ok = multiply_stages<PARTS, EPI, 1>(t, tmem_base, smem, full, empty, tfull, tempty, ring, acc, abort_flag);
+          ok = multiply_stages<PARTS, EPI, 1>(t, kept, tmem_base, smem, full, empty, tfull, tempty, ring, acc,
+                                              abort_flag);
         else
-          ok = multiply_stages<PARTS, EPI, 0>(t, tmem_base, smem, full, empty, tfull, tempty, ring, acc, abort_flag);
+          ok = multiply_stages<PARTS, EPI, 0>(t, kept, tmem_base, smem, full, empty, tfull, tempty, ring, acc,
+                                              abort_flag);
       }
       if (lane == 0) {
         if (!ok) {
@@ -893,7 +942,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
     const int warp_row = (int)rank * 128 + quarter * 32;
     BlockOut block{smem + kStageBytes + (warp - 2) * kOutBytes, lane, 0, false};
     const uint32_t release[2] = {at_leader(&tempty[0]), at_leader(&tempty[1])};
-    constexpr int kChunk = chunk_of<PARTS, EPI>();
+    constexpr bool kChunks = PARTS == 2 || EPI == kStats;
+    const int chunk = chunk_of<PARTS, EPI>(kept);
     Ring acc;
     bool ok = true;
     for (int index = pair; index < tiles && ok; index += pairs) {
@@ -906,11 +956,11 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
         if (lane == 0) arrive_at(release[acc.at]);
         acc.next(2);
       };
-      if constexpr (kChunk > 0) {
+      if constexpr (kChunks) {
         float total[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) total[j] = 0.f;
-        for (int first = t.first; first < t.last; first += kChunk) {
+        for (int first = t.first; first < t.last; first += chunk) {
           if (!(ok = warp_wait(&tfull[acc.at], acc.phase, abort_flag))) break;
           fence_after();
 #pragma unroll
@@ -974,19 +1024,33 @@ __device__ __forceinline__ void merge(float& top, float& sum, float top2, float 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
-// The logits of up to ROWS kept float32 rows (the groups of blockIdx.y) reduced to statistics: bound by reading the head
-// once. A warp takes BATCH rows of the head at a time, 16 bytes a lane and row, against the hidden rows in shared
-// memory, then adds its BATCH x ROWS sums across its lanes by halving: lane l ends with the sum of index l / (32 / (BATCH
-// x ROWS)).
-template <int ROWS, int BATCH>
-__global__ void __launch_bounds__(kFewThreads) few_kernel(const float* hidden, int64_t stride, const float* head,
+// The logits of up to ROWS kept rows (the groups of blockIdx.y) reduced to statistics: bound by reading the head once. A
+// warp takes BATCH rows of the head at a time, 16 bytes a lane and row, against the hidden rows in shared memory
+// (float32, in planes of 16-byte pieces, so that neighbouring lanes read neighbouring pieces), then adds its BATCH x ROWS
+// sums across its lanes by halving: lane l ends with the sum of index l / (32 / (BATCH x ROWS)).
+template <typename T>
+__device__ __forceinline__ void widen(uint4 bits, float (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (sizeof(T) == 4) {
+      x[j] = __uint_as_float(w[j]);
+    } else {
+      x[2 * j] = __uint_as_float(w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  }
+}
+
+template <typename T, int ROWS, int BATCH>
+__global__ void __launch_bounds__(kFewThreads) few_kernel(const T* hidden, int64_t stride, const T* head,
                                                           const int64_t* targets, int64_t ignore, int n, int d, int vocab,
                                                           float2* stats, int64_t n_pad, float* picked, float* losses,
                                                           State s) {
-  constexpr int kSums = ROWS * BATCH;
+  constexpr int kVector = 16 / sizeof(T), kPlanes = kVector / 4, kSums = ROWS * BATCH;
   static_assert(kSums <= 32 && (kSums & (kSums - 1)) == 0, "one sum a lane at most");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  float* rows = reinterpret_cast<float*>(smem_raw);                       // [ROWS][d]
+  float* rows = reinterpret_cast<float*>(smem_raw);                       // [ROWS][kPlanes][d / kPlanes]
   __shared__ int row_of[32], target_of[32], kept_rows;
   __shared__ float2 shared[kFewWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = blockIdx.y * ROWS;
@@ -1022,9 +1086,12 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const float* hidden, i
   if (first >= kept) return;
   for (int i = threadIdx.x; i < ROWS * d; i += kFewThreads) {
     const int r = i / d, c = i % d;
-    const float v = first + r < kept ? hidden[row_of[first + r] * stride + c] : 0.f;
-    rows[i] = v;
-    if (blockIdx.x == 0 && first + r < kept) s.raw[(int64_t)first * d + i] = v;
+    const T v = first + r < kept ? hidden[row_of[first + r] * stride + c] : from_f<T>(0.f);
+    rows[(r * kPlanes + c / 4 % kPlanes) * (d / kPlanes) + c / kVector * 4 + c % 4] = to_f<T>(v);
+    if (blockIdx.x == 0 && first + r < kept) {
+      if constexpr (sizeof(T) == 4) s.raw[(int64_t)first * d + i] = v;
+      else static_cast<T*>(s.hidden[0])[(int64_t)first * d + i] = v;
+    }
   }
   __syncthreads();
 
@@ -1036,23 +1103,28 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const float* hidden, i
   for (int v0 = (blockIdx.x * kFewWarps + warp) * BATCH; v0 < vocab; v0 += step) {
     float acc[kSums] = {};
 #pragma unroll 2
-    for (int c = lane * 4; c < d; c += 128) {
-      float4 w[BATCH];
+    for (int c = lane * kVector; c < d; c += 32 * kVector) {
+      uint4 bits[BATCH];
 #pragma unroll
       for (int b = 0; b < BATCH; ++b)
-        w[b] = __ldcs(reinterpret_cast<const float4*>(head + (int64_t)min(v0 + b, vocab - 1) * d + c));
+        bits[b] = __ldcs(reinterpret_cast<const uint4*>(head + (int64_t)min(v0 + b, vocab - 1) * d + c));
+      float w[BATCH][kVector];
 #pragma unroll
-      for (int r = 0; r < ROWS; ++r) {
-        const float4 h = *reinterpret_cast<const float4*>(rows + r * d + c);
+      for (int b = 0; b < BATCH; ++b) widen<T>(bits[b], w[b]);
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b) {
-          float& a = acc[b * ROWS + r];
-          a = fmaf(h.x, w[b].x, a);
-          a = fmaf(h.y, w[b].y, a);
-          a = fmaf(h.z, w[b].z, a);
-          a = fmaf(h.w, w[b].w, a);
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int p = 0; p < kPlanes; ++p) {
+          const float4 h = *reinterpret_cast<const float4*>(rows + (r * kPlanes + p) * (d / kPlanes) + c / kPlanes);
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) {
+            float& a = acc[b * ROWS + r];
+            a = fmaf(h.x, w[b][4 * p], a);
+            a = fmaf(h.y, w[b][4 * p + 1], a);
+            a = fmaf(h.z, w[b][4 * p + 2], a);
+            a = fmaf(h.w, w[b][4 * p + 3], a);
+          }
         }
-      }
     }
 #pragma unroll
     for (int o = 16, count = kSums; o > 0; o >>= 1) {
@@ -1129,9 +1201,8 @@ __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* sta
     }
     const int mine = blockIdx.x * 32 + warp;
     if (lane == 0 && mine < kept) {
-      const float lse = v.x + logf(v.y);
-      s.lse[mine] = lse;
-      losses[s.row_of[mine]] = lse - picked[mine];
+      s.sums[mine] = v;
+      losses[s.row_of[mine]] = (v.x - picked[mine]) + logf(v.y);
     }
   }
   if (reduction == HFFN_REDUCE_NONE) return;
@@ -1306,12 +1377,12 @@ static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_
 
 constexpr int kFewBlocks = 148 * 3;    // of the few-row kernel: 24 warps an SM
 
-template <int ROWS, int BATCH>
-static int launch_few(const float* hidden, int64_t stride, const float* head, const int64_t* targets, int64_t ignore,
-                      int n, int d, int vocab, float2* stats, int64_t n_pad, float* picked, float* losses, const State& s,
+template <typename T, int ROWS, int BATCH>
+static int launch_few(const T* hidden, int64_t stride, const T* head, const int64_t* targets, int64_t ignore, int n,
+                      int d, int vocab, float2* stats, int64_t n_pad, float* picked, float* losses, const State& s,
                       int blocks, cudaStream_t st) {
-  HFFN_TRY((allow_shared_memory<few_kernel<ROWS, BATCH>>((int)kFewBytes)));
-  few_kernel<ROWS, BATCH><<<dim3(blocks, (unsigned)ceil_div(n, ROWS)), kFewThreads, ROWS * d * 4, st>>>(
+  HFFN_TRY((allow_shared_memory<few_kernel<T, ROWS, BATCH>>((int)kFewBytes)));
+  few_kernel<T, ROWS, BATCH><<<dim3(blocks, (unsigned)ceil_div(n, ROWS)), kFewThreads, ROWS * d * 4, st>>>(
       hidden, stride, head, targets, ignore, n, d, vocab, stats, n_pad, picked, losses, s);
   return launch_status("linear_ce few rows");
 }
@@ -1370,7 +1441,8 @@ static int measuring_blocks(int vocab, int d) {
 
 template <typename T>
 static int forward(const void* hidden, int64_t stride, const void* weight, const int64_t* targets, int64_t ignore,
-                   int reduction, float* loss, void* state, void* work, int n, int d, int vocab, cudaStream_t st) {
+                   int reduction, bool for_backward, float* loss, void* state, void* work, int n, int d, int vocab,
+                   cudaStream_t st) {
   constexpr int PARTS = sizeof(T) / 2;
   constexpr int dtype = PARTS == 2 ? HFFN_F32 : HFFN_BF16;
   const ForwardWork w = forward_work(work, n, vocab);
@@ -1385,25 +1457,22 @@ static int forward(const void* hidden, int64_t stride, const void* weight, const
   const T *rows = static_cast<const T*>(hidden), *head = static_cast<const T*>(weight);
   int parts = 0;
   if (is_few(dtype, n, d)) {
-    if constexpr (PARTS == 2) {
-      parts = (int)std::min<int64_t>(kFewBlocks, ceil_div(vocab, kFewWarps * 4));
-      const int each = few_rows(n);
-      auto few = each == 1   ? launch_few<1, 8>
-                 : each == 2 ? launch_few<2, 8>
-                 : each == 4 ? launch_few<4, 4>
-                             : launch_few<kFewRows, 4>;
-      HFFN_TRY(few(rows, stride, head, targets, ignore, n, d, vocab, w.stats, e.n_pad, w.picked, losses, e.s, parts, st));
-    }
+    parts = (int)std::min<int64_t>(kFewBlocks, ceil_div(vocab, kFewWarps * 4));
+    auto few = launch_few<T, PARTS == 1 ? 1 : kFewRows, PARTS == 1 ? 8 : 4>;
+    if constexpr (PARTS == 2)
+      if (few_rows(dtype, n) < kFewRows) few = launch_few<T, kFewRows / 2, 4>;
+    HFFN_TRY(few(rows, stride, head, targets, ignore, n, d, vocab, w.stats, e.n_pad, w.picked, losses, e.s, parts, st));
   } else {
     const int span = (int)std::max<int64_t>(16, ceil_div(n, 512)), gather = (int)ceil_div(n, span);
     const bool aligned = (reinterpret_cast<uintptr_t>(hidden) & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
     if (PARTS == 2 && cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
-    const int measure = PARTS == 2 ? measuring_blocks(vocab, d) : 0;
+    const int measure = PARTS == 2 && for_backward ? measuring_blocks(vocab, d) : 0;
     gather_kernel<T><<<gather + measure, kGatherThreads, 0, st>>>(rows, stride, head, targets, ignore, n, d, vocab, span,
                                                                   gather, aligned, losses, e.s);
     if constexpr (PARTS == 2)
       launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, rows, stride, aligned,
-                                head, d, vocab, e.s);
+                                head, d, vocab, !for_backward, e.s);
+    if (PARTS == 2 && !for_backward) e.head_inverse = e.s.inverse;
     Maps maps;
     HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
     HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), true, st)));
@@ -1420,6 +1489,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
                     void* state, void* work, int n, int d, int vocab, cudaStream_t st) {
   constexpr int PARTS = sizeof(T) / 2;
   constexpr int dtype = PARTS == 2 ? HFFN_F32 : HFFN_BF16;
+  if (grad_hidden == nullptr && grad_weight == nullptr) return HFFN_OK;
   const BackwardWork w = backward_work(work, dtype, n, d, vocab);
   const int width = piece_width(dtype, n, vocab), splits = hidden_splits(dtype, n, d, vocab);
   Args e = {};
@@ -1435,7 +1505,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       if (cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
       measure_kernel<<<1 + measuring_blocks(vocab, d), kGatherThreads, 0, st>>>(values, d, vocab, e.s);
       launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, (const float*)nullptr,
-                                (int64_t)0, true, values, d, vocab, e.s);
+                                (int64_t)0, true, values, d, vocab, false, e.s);
       prepared = true;
     }
   }
@@ -1539,8 +1609,8 @@ int64_t hffn_linear_ce_backward_workspace(int dtype, int64_t n, int32_t d, int32
 }
 
 int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
-                           const int64_t* targets, int64_t ignore_index, int reduction, float* loss, void* state,
-                           void* work, int64_t n, int32_t d, int32_t vocab, void* stream) {
+                           const int64_t* targets, int64_t ignore_index, int reduction, int for_backward, float* loss,
+                           void* state, void* work, int64_t n, int32_t d, int32_t vocab, void* stream) {
   HFFN_TRY(ce::check(dtype, n, d, vocab));
   HFFN_REQUIRE(reduction == HFFN_REDUCE_NONE || reduction == HFFN_REDUCE_MEAN || reduction == HFFN_REDUCE_SUM,
                "unknown reduction %d", reduction);
@@ -1551,8 +1621,8 @@ int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride,
   HFFN_TRY(bind_stream_device(stream));
   HFFN_TRY(ce::bind_context());
   auto run = dtype == HFFN_F32 ? ce::forward<float> : ce::forward<__nv_bfloat16>;
-  return run(hidden, hidden_stride, weight, targets, ignore_index, reduction, loss, state, work, (int)n, d, vocab,
-             static_cast<cudaStream_t>(stream));
+  return run(hidden, hidden_stride, weight, targets, ignore_index, reduction, for_backward != 0, loss, state, work,
+             (int)n, d, vocab, static_cast<cudaStream_t>(stream));
 }
 
 int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const float* grad_loss, void* grad_hidden,

@@ -45,7 +45,7 @@ def _sizes(code: int, n: int, d: int, vocab: int) -> tuple[int, int, int]:
             native.lib.hffn_linear_ce_backward_workspace(code, n, d, vocab))
 
 
-def _forward(hidden, weight, targets, ignore_index, reduction):
+def _forward(hidden, weight, targets, ignore_index, reduction, for_backward=True):
     """The losses of hidden [N, d] (any row stride) and the state that ``_backward`` reads."""
     n, d = hidden.shape
     vocab, device, code = weight.shape[0], hidden.device, DTYPES[hidden.dtype]
@@ -54,12 +54,17 @@ def _forward(hidden, weight, targets, ignore_index, reduction):
     targets = targets.contiguous()
     state_bytes, work_bytes, _ = _sizes(code, n, d, vocab)
     loss = torch.empty(n if reduction == "none" else (), device=device)
-    state = torch.empty(state_bytes, dtype=torch.uint8, device=device)
-    work = torch.empty(work_bytes, dtype=torch.uint8, device=device)
+    if for_backward:
+        state = torch.empty(state_bytes, dtype=torch.uint8, device=device)
+        work = torch.empty(work_bytes, dtype=torch.uint8, device=device)
+        addresses = state.data_ptr(), work.data_ptr()
+    else:                                     # one buffer; the state's size is a multiple of 256
+        state = torch.empty(state_bytes + work_bytes, dtype=torch.uint8, device=device)
+        addresses = state.data_ptr(), state.data_ptr() + state_bytes
     with native.on_device(device.index):
         native.check(native.lib.hffn_linear_ce_forward(
             code, hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), targets.data_ptr(), ignore_index,
-            native.REDUCE_CODES[reduction], loss.data_ptr(), state.data_ptr(), work.data_ptr(), n, d, vocab,
+            native.REDUCE_CODES[reduction], for_backward, loss.data_ptr(), *addresses, n, d, vocab,
             native.raw_stream(device.index)), "hffn_linear_ce_forward")
     return loss, state
 
@@ -115,7 +120,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
         loss = LinearCrossEntropyFunction.apply(rows, weight, flat, int(ignore_index), reduction)
     else:
-        loss, _ = _forward(rows, weight, flat, int(ignore_index), reduction)
+        loss, _ = _forward(rows, weight, flat, int(ignore_index), reduction, for_backward=False)
     return loss.view(targets.shape) if reduction == "none" and hidden.dim() != 2 else loss
 
 

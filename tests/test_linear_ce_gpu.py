@@ -109,6 +109,9 @@ def check(h, w, targets, reduction="none", seed=3, ignore_index=IGNORE):
         within(loss.detach(), (total, bound + U * total.abs()), "loss")
     within(dh, expected_dh, "grad_hidden")
     within(dw, expected_dw, "grad_weight")
+    with torch.no_grad():                                  # without a backward
+        scored = linear_cross_entropy(h, w, targets, ignore_index=ignore_index, reduction="none")
+    within(scored, expected_losses, "scored losses")
     return loss.detach(), dh, dw
 
 

@@ -28,7 +28,7 @@ def test_linear_ce_entries_refuse_bad_arguments():
 
     def forward(dtype=n.F32, hidden=16, stride=16, weight=16, targets=16, reduction=0, loss=16, buffer=16, rows=4, d=16,
                 vocab=10):
-        return lib.hffn_linear_ce_forward(dtype, hidden, stride, weight, targets, -100, reduction, loss, buffer, buffer,
+        return lib.hffn_linear_ce_forward(dtype, hidden, stride, weight, targets, -100, reduction, 1, loss, buffer, buffer,
                                           rows, d, vocab, None)
 
     for bad in (dict(dtype=5), dict(hidden=None), dict(weight=None), dict(targets=None), dict(loss=None),
