@@ -33,7 +33,7 @@ class _List:
     list: a model has hundreds of gradients, and this is the host's cost of a call."""
 
     def __init__(self, tensors, what: str) -> None:
-        tensors = self.tensors = list(tensors)
+        tensors = self.tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
         try:
             types = [_CODES[t.dtype] for t in tensors]
             devices = set(map(torch.Tensor.get_device, tensors))
@@ -65,8 +65,8 @@ def _buffers(tensors: _List):
 
 
 def grad_norm(tensors) -> torch.Tensor:
-    """The 2-norm over every entry of ``tensors`` (float32 / bfloat16, dense, on one CUDA device): a float32 scalar on
-    that device, computed in float64 and rounded once. An empty list has norm 0 (on the current device)."""
+    """The 2-norm over every entry of ``tensors`` (one or many, float32 / bfloat16, dense, on one CUDA device): a float32
+    scalar on that device, computed in float64 and rounded once. An empty list has norm 0 (on the current device)."""
     tensors = _List(tensors, "tensors")
     norm, work = _buffers(tensors)
     with native.on_device(tensors.device):

@@ -132,6 +132,18 @@ def test_zero_limit_zero_gradients_and_nothing():
     assert float(clip_grad_norm(empty, 1.0)) == 0.0
 
 
+def test_a_tensor_alone():
+    from hffn_b200.grad_clip import clip_grad_norm, grad_norm
+    x = make([(30, 7)], torch.float32, 5)[0]
+    before = x.clone()
+    norm = norm64([x])
+    assert abs(float(grad_norm(x)) - norm) <= 2 * U * norm
+    clip_grad_norm(x, norm / 5)
+    check_scaled([x], [before], norm, norm / 5)
+    point = torch.tensor(-3.0, device="cuda")
+    assert float(grad_norm(point)) == 3.0
+
+
 def test_same_bits_streams_and_capture():
     from hffn_b200.grad_clip import clip_grad_norm
     tensors = make([(2000, 300), (77,), (5, 5)], torch.float32, 4)

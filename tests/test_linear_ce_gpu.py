@@ -123,7 +123,7 @@ def no_wait_ran_out():
 
 
 BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-SHAPES = [(1, 8, 1), (1, 64, 2), (2, 72, 7), (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
+SHAPES = [(9000, 8, 300), (40, 4104, 600), (3, 8, 140001), (2, 32768, 40), (1, 8, 1), (1, 64, 2), (2, 72, 7), (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
           (256, 512, 1000), (257, 1024, 2049), (700, 328, 4099), (1, 1024, 50304), (9, 2048, 5001), (1021, 768, 3001)]
 
 
@@ -408,6 +408,72 @@ def test_gradients_outside_autograd(dtype):
         linear_cross_entropy_gradients(h, w, t, c[:5], reduction="none")
     with pytest.raises(ValueError):
         linear_cross_entropy_gradients(h, w, t, c)
+
+
+@pytest.mark.parametrize("n", [1, 20])
+def test_offsets_past_32_bits(n):
+    """A head of 2.2e9 entries: the losses against float32 sums over the head in stretches (whose own errors are far
+    below the bound), and the last rows of its gradient, where the targets lie."""
+    from hffn_b200.losses import linear_cross_entropy
+    v, d = 1_060_003, 2056
+    g = torch.Generator(device="cuda").manual_seed(24)
+    w = torch.empty(v, d, dtype=torch.bfloat16, device="cuda").normal_(0, 2 / math.sqrt(d), generator=g)
+    h = torch.randn(n, d, generator=g, device="cuda").bfloat16()
+    t = torch.arange(v - n, v, device="cuda")
+    z = torch.cat([h.double() @ part.double().T for part in w.split(100_000)], 1)
+    lse = torch.logsumexp(z, 1)
+    dz = acc(d) * max(float((h.double().abs() @ part.double().abs().T).max()) for part in w.split(100_000))
+    e = 2 * dz + 8 * U * (float(z.abs().max()) + 1 + math.log(v))
+    h.requires_grad_(True), w.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    expected = lse - z[torch.arange(n), t]
+    assert float((losses.detach().double() - expected).abs().max()) <= e + 2 * U * float(lse.max() + z.abs().max())
+    dh, dw = torch.autograd.grad(losses.sum(), (h, w))
+    h, w = h.detach(), w.detach()
+    p = (z[:, -1000:] - lse[:, None]).exp()
+    p[torch.arange(n), t - (v - 1000)] -= 1
+    exact = p.T @ h.double()
+    bound = (2 * 2.0 ** -8 + 2 * math.expm1(e)) * (p.abs().T @ h.double().abs()) + 1e-30
+    assert bool(((dw[-1000:].double() - exact).abs() <= bound).all())
+    assert bool(torch.isfinite(dw[:: 1000]).all()) and bool(torch.isfinite(dh).all())
+    del z, dw
+    torch.cuda.empty_cache()
+
+
+@BOTH
+def test_one_token_of_every_kind(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(1, 64, 300, dtype, seed=25)
+    check(h, w, t)
+    for bad, expected in ((IGNORE, 0.0), (300, math.nan), (-7, math.nan)):
+        hg, wg = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        for reduction in ("none", "mean", "sum"):
+            loss = linear_cross_entropy(hg, wg, torch.full_like(t, bad), reduction=reduction)
+            dh, dw = torch.autograd.grad(loss.sum(), (hg, wg))
+            assert bool((dh == 0).all()) and bool((dw == 0).all())
+            assert bool(torch.isnan(loss).all()) if math.isnan(expected) else bool((loss == expected).all())
+    h[0, 3] = float("inf")
+    assert not bool(torch.isfinite(linear_cross_entropy(h, w, t)))
+
+
+@BOTH
+def test_two_backwards_of_one_forward(dtype):
+    from hffn_b200.losses import linear_cross_entropy
+    for n in (3, 70):
+        h, w, t = make(n, 64, 900, dtype, seed=26)
+        h.requires_grad_(True), w.requires_grad_(True)
+        loss = linear_cross_entropy(h, w, t)
+        first = torch.autograd.grad(loss, (h, w), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(loss, (h, w))))
+
+
+def test_second_derivatives_are_refused():
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(20, 64, 300, torch.float32)
+    h.requires_grad_(True)
+    (dh,) = torch.autograd.grad(linear_cross_entropy(h, w, t), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dh.sum().backward()
 
 
 def test_from_a_thread_that_has_made_no_cuda_call():
