@@ -582,11 +582,12 @@ struct RowEpilogue {
   int target;
   float factor;             // of the accumulators
   float top, sum;           // kStats
+  float4 inverse;           // kStats with a scale for each row of the head: of this lane's 4 of the warp's 128 columns
   float2 sums;              // kGrad
   float lse2, c;
 
   __device__ __forceinline__ RowEpilogue(const Maps& maps_, const Args& args, BlockOut& out_, const Tile& tile,
-                                         int warp_row, int kept)
+                                         int warp_row, int first_col, int kept)
       : maps(maps_), e(args), out(out_), t(tile) {
     first_row = t.m * kTile + warp_row;
     row = first_row + out.lane;
@@ -600,10 +601,17 @@ struct RowEpilogue {
       live = row < kept;
       target = live ? e.s.target[row] : -1;
       if (PARTS == 2)
-        factor = power_of_two(-scale_exponent(e.s.largest[0]) -
-                              (EPI == kStats && e.head_inverse ? 0 : scale_exponent(e.s.largest[1])));
+        // within float32's range: logits that it cuts off there are zero or overflow anyway
+        factor = power_of_two(
+            max(-126, min(127, -scale_exponent(e.s.largest[0]) -
+                                   (EPI == kStats && e.head_inverse ? 0 : scale_exponent(e.s.largest[1])))));
       top = -INFINITY;
       sum = 0.f;
+      if (PARTS == 2 && EPI == kStats && e.head_inverse) {
+        const int col = first_col + 4 * out.lane;       // the array is padded to a multiple of 64
+        inverse = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (col < e.vocab) inverse = __ldg(reinterpret_cast<const float4*>(e.head_inverse + col));
+      }
       if (EPI == kGrad) {
         sums = live ? e.s.sums[row] : make_float2(0.f, 1.f);
         lse2 = (sums.x + logf(sums.y)) * kLog2e;
@@ -613,23 +621,28 @@ struct RowEpilogue {
     }
   }
 
+  // The sums are complete: the columns' scales where every lane reads them (nothing leaves through this memory here).
+  __device__ __forceinline__ void begin() {
+    if constexpr (PARTS == 2 && EPI == kStats) {
+      if (!e.head_inverse) return;
+      __syncwarp();
+      reinterpret_cast<float4*>(out.base)[out.lane] = inverse;
+      __syncwarp();
+    }
+  }
+
   __device__ __forceinline__ void columns(float (&v)[32], int col) {
-    if constexpr (PARTS == 2) {
+    if constexpr (PARTS == 2 && EPI != kStats) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= factor;
     }
     if constexpr (EPI == kStats) {
       if (PARTS == 2 && e.head_inverse) {
-        if (col + 32 <= e.vocab) {
+        const float* scales = reinterpret_cast<const float*>(out.base) + (col & 127);
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 x = __ldg(reinterpret_cast<const float4*>(e.head_inverse + col + j));
-            v[j] *= x.x, v[j + 1] *= x.y, v[j + 2] *= x.z, v[j + 3] *= x.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col + j < e.vocab) v[j] *= __ldg(e.head_inverse + col + j);
+        for (int j = 0; j < 32; j += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(scales + j);
+          v[j] *= x.x, v[j + 1] *= x.y, v[j + 2] *= x.z, v[j + 3] *= x.w;
         }
       }
       if (col + 32 > e.vocab) {
@@ -641,18 +654,21 @@ struct RowEpilogue {
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (at == j) e.picked[row] = v[j];
+          if (at == j) e.picked[row] = v[j] * factor;
       }
-      float most = top;
+      // `factor` is a power of two, so it goes into the exponents' and the maximum's multiplications unrounded
+      float most = v[0];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) most = fmaxf(most, v[j]);
+      for (int j = 1; j < 32; ++j) most = fmaxf(most, v[j]);
+      most = fmaxf(top, most * factor);
+      const float factor2 = factor * kLog2e;
       // a row of -inf so far has nothing to rescale; NaN logits reach the sum through their exponentials. The rounding
       // of `base` (1e-6 of a logit of 16) is the same in all 32 exponents: it is taken out of their sum.
       const bool none = most == -INFINITY;
       const float base = none ? 0.f : most * kLog2e;
       float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) part[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -base));
+      for (int j = 0; j < 32; ++j) part[j & 3] += exp2_fast(fmaf(v[j], factor2, -base));
       const float more = (part[0] + part[1]) + (part[2] + part[3]);
       sum = none ? sum + more
                  : fmaf(sum, exp2_fast((top - most) * kLog2e), more * exp2_fast(-fmaf(most, kLog2e, -base)));
@@ -952,8 +968,8 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
     bool ok = true;
     for (int index = pair; index < tiles && ok; index += pairs) {
       const Tile t = tile_of<EPI>(index, extent, e);
-      RowEpilogue<PARTS, EPI> out(maps, e, block, t, warp_row, kept);
       const int col = t.n * kTile + half * 128;
+      RowEpilogue<PARTS, EPI> out(maps, e, block, t, warp_row, col, kept);
       auto release_buffer = [&] {
         fence_before();
         __syncwarp();
@@ -977,6 +993,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
           release_buffer();
         }
         if (!ok) break;
+        out.begin();
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v[32];

@@ -242,6 +242,13 @@ def test_logits_of_every_size(size, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("h_size,w_size", [(0.0, 1.0), (1.0, 0.0), (0.0, 0.0), (1e-25, 1e-25), (1e25, 1e-25), (1e-25, 1e25)])
+def test_operands_of_every_size(h_size, w_size, dtype):
+    h, w, t = make(60, 128, 700, dtype, seed=27)
+    check((h.float() * h_size).to(dtype), (w.float() * w_size).to(dtype), t)
+
+
+@BOTH
 def test_rows_of_very_different_sizes(dtype):
     """Hidden rows, head rows and upstream gradients over several decades."""
     h, w, t = make(130, 128, 600, dtype, seed=10)
