@@ -15,16 +15,18 @@
 // that an SM takes 32 KB from L2 per 64 values of K for 256 x 256 x 64 products of the pair. Two accumulator buffers let
 // the epilogue of one tile run under the products of the next.
 //
-// Types. bfloat16: products of the inputs as they are; g, c_t included, is held in bfloat16 (off by at most 2^-8 of an
-// entry, as the gradients' own storage). float32: three fp16 products per product, of operands held as two fp16 parts (hi
-// = rn(x 2^e), lo = rn(x 2^e - hi); hi hi + hi lo + lo hi, the rest is below 2^-22), 2^e one power of two per operand that
-// brings its largest finite entry to [2^14, 2^15): entries down to 2^-17 of the largest keep 22 bits, smaller ones are
-// held to 2^-39 of it. One scale per operand, not per row, because each of h, w and g is summed over its rows in one of
-// the products. g holds 2^14 (p - [v = target]); c_t is applied in float32 afterwards (dh: per row; dw: one factor, or
-// rows of h scaled by their c_t beforehand where they differ). A forward without a backward takes a scale for each row of
-// the head instead, which saves the pass that finds the largest entry (2048 x 1024 x 50304: 50 of 600 us). Sums: the
-// tensor core's float32 accumulation truncates at every step, so what ends in float32 (float32 gradients, losses) is
-// summed in registers from accumulators of few steps each (chunk_of).
+// Types. bfloat16: products of the inputs as they are; g is held in bfloat16, off by at most 2^-8 of an entry, as the
+// gradients' own storage. It holds p - [v = target] where all tokens have one c, which is applied to dh and dw in float32
+// (the target's entry of a token that is not well predicted, the largest, is then close to -1, which is exact), and c
+// with it where they differ (a c h in bfloat16 beside it would round twice). float32: three fp16 products per product, of
+// operands held as two fp16 parts (hi = rn(x 2^e), lo = rn(x 2^e - hi); hi hi + hi lo + lo hi, the rest is below 2^-22),
+// 2^e one power of two per operand that brings its largest finite entry to [2^14, 2^15): entries down to 2^-17 of the
+// largest keep 22 bits, smaller ones are held to 2^-39 of it. One scale per operand, not per row, because each of h, w
+// and g is summed over its rows in one of the products. g holds 2^14 (p - [v = target]); c_t is applied in float32
+// afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). A float32
+// forward without a backward takes a scale for each row of the head instead, which saves the pass that finds the largest
+// entry (2048 x 1024 x 50304: 50 of 600 us). Sums: the tensor core's float32 accumulation truncates at every step, so
+// what ends in float32 (float32 gradients, losses) is summed in registers from accumulators of few steps each (chunk_of).
 //
 // Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 252 us, g 258 us, dh and dw 534 us (1.6 to 1.7
 // PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 204, 225 and 438 us (89, 80 and 93 %).
@@ -397,7 +399,7 @@ struct Args {
   const float* head_inverse;   // kStats, float32: of each row of the head (NULL: one scale for all)
   int add;                 // kGradients: dh adds to its slots (a later piece)
   const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
-  int dw_upstream;                   // float32: dw's rows lack their c, which is the same for all
+  int dw_upstream;                   // dw's rows lack their c, which is the same for all
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -593,8 +595,8 @@ struct RowEpilogue {
     row = first_row + out.lane;
     factor = 1.f;
     if constexpr (EPI == kGradients) {
-      if (PARTS == 2 && t.job == 1) {
-        factor = power_of_two(-14 - scale_exponent(*e.dw_rows_largest));
+      if (t.job == 1) {
+        if (PARTS == 2) factor = power_of_two(-14 - scale_exponent(*e.dw_rows_largest));
         if (e.dw_upstream && kept > 0) factor *= e.upstream.of(e.s, 0, kept);
       }
     } else {
@@ -616,7 +618,7 @@ struct RowEpilogue {
         sums = live ? e.s.sums[row] : make_float2(0.f, 1.f);
         lse2 = (sums.x + logf(sums.y)) * kLog2e;
         sums.y = 1.f / sums.y;
-        c = PARTS == 2 ? 16384.f : live ? e.upstream.of(e.s, row, kept) : 0.f;
+        c = PARTS == 2 ? 16384.f : live && e.upstream.reduction == HFFN_REDUCE_NONE ? e.upstream.of(e.s, row, kept) : 1.f;
       }
     }
   }
@@ -632,7 +634,7 @@ struct RowEpilogue {
   }
 
   __device__ __forceinline__ void columns(float (&v)[32], int col) {
-    if constexpr (PARTS == 2 && EPI != kStats) {
+    if constexpr (EPI == kGradients || (PARTS == 2 && EPI == kGrad)) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= factor;
     }
@@ -1256,8 +1258,9 @@ __global__ void __launch_bounds__(256) scatter_kernel(State s, const float* slot
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (t >= n) return;
   const int at = s.place_of[t];
-  float factor = 1.f;
-  if (sizeof(T) == 4 && at >= 0) factor = upstream.of(s, at, *s.kept) * power_of_two(-14 - scale_exponent(s.largest[1]));
+  float factor = 1.f;      // what g lacks
+  if (at >= 0 && (sizeof(T) == 4 || upstream.reduction != HFFN_REDUCE_NONE)) factor = upstream.of(s, at, *s.kept);
+  if (sizeof(T) == 4) factor *= power_of_two(-14 - scale_exponent(s.largest[1]));
   for (int i = 4 * lane; i < d; i += 128) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= 0)
@@ -1531,21 +1534,18 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
     }
   }
   const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
-  if (PARTS == 2) {
-    e.dw_rows_largest = e.s.largest;
-    if (reduction != HFFN_REDUCE_NONE) {
-      e.dw_upstream = 1;
-    } else if (grad_weight != nullptr) {
-      e.dw_rows_largest = w.largest;
-      rows[0] = w.rows[0];
-      rows[1] = w.rows[1];
-      if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
-      __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
-      const unsigned blocks = (unsigned)(e.n_pad / 8);
-      scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
-      launch_next<scaled_rows_kernel<true>>(blocks, 256, 0, st, e.s, e.upstream, w.largest, hi, lo, d);
-      prepared = true;
-    }
+  e.dw_rows_largest = e.s.largest;
+  e.dw_upstream = reduction != HFFN_REDUCE_NONE;
+  if (PARTS == 2 && reduction == HFFN_REDUCE_NONE && grad_weight != nullptr) {
+    e.dw_rows_largest = w.largest;
+    rows[0] = w.rows[0];
+    rows[1] = w.rows[1];
+    if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
+    const unsigned blocks = (unsigned)(e.n_pad / 8);
+    __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
+    scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
+    launch_next<scaled_rows_kernel<true>>(blocks, 256, 0, st, e.s, e.upstream, w.largest, hi, lo, d);
+    prepared = true;
   }
   const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
   const int64_t row_tiles = ceil_div(n, kTile), wide = ceil_div(d, kTile);

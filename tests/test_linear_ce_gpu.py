@@ -5,8 +5,9 @@ the storage type (bfloat16 2^-8; float32: the operands of the products are held 
 representation and dropped low-by-low product are within r = 2^-20 of a product, then rounded once to float32).
 - A product summed over k terms in float32 is within acc(k) = (k / 16 + 32) 2^-23 of the sum of its terms' absolute
   values (the tensor core adds 16 products at a time and truncates; one step each, and the sums within one add).
-- A logit is within dz = (acc(d) + [float32: r]) sum_i |h_i w_i| of the exact one; every exponential's argument and the log sum
-  are within the largest dz of a row plus rounding of a value of size |z|: e_t = 2 max_v dz + 8 u (max |z| + 1 + log V).
+- A logit is within dz = (acc(d) + [float32: r]) sum_i |h_i w_i| of the exact one; every exponential's argument and the
+  log sum are within the largest dz of a row plus rounding of a value of size |z|: e_t = 2 max_v dz + 8 u (max |z| + 1
+  + log V).
 - loss_t is within e_t + u (|lse| + |z|).
 - g = c (p - [target]) is within |c| p (e^{e_t} - 1 + 2^-20) + r |g| (its storage) of the exact one, and a gradient
   sum_k g x is within sum_k |delta g| |x| + (acc(k) + [float32: r]) sum_k |g x| + r |result|.
@@ -123,7 +124,8 @@ def no_wait_ran_out():
 
 
 BOTH = pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-SHAPES = [(9000, 8, 300), (40, 4104, 600), (3, 8, 140001), (2, 32768, 40), (1, 8, 1), (1, 64, 2), (2, 72, 7), (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
+SHAPES = [(9000, 8, 300), (40, 4104, 600), (3, 8, 140001), (2, 32768, 40), (1, 8, 1), (1, 64, 2), (2, 72, 7),
+          (46, 128, 1024), (31, 136, 255), (64, 64, 256), (255, 200, 257),
           (256, 512, 1000), (257, 1024, 2049), (700, 328, 4099), (1, 1024, 50304), (9, 2048, 5001), (1021, 768, 3001)]
 
 
@@ -242,7 +244,8 @@ def test_logits_of_every_size(size, dtype):
 
 
 @BOTH
-@pytest.mark.parametrize("h_size,w_size", [(0.0, 1.0), (1.0, 0.0), (0.0, 0.0), (1e-25, 1e-25), (1e25, 1e-25), (1e-25, 1e25)])
+@pytest.mark.parametrize("h_size,w_size", [(0.0, 1.0), (1.0, 0.0), (0.0, 0.0), (1e-25, 1e-25), (1e25, 1e-25),
+                                           (1e-25, 1e25)])
 def test_operands_of_every_size(h_size, w_size, dtype):
     h, w, t = make(60, 128, 700, dtype, seed=27)
     check((h.float() * h_size).to(dtype), (w.float() * w_size).to(dtype), t)
@@ -363,11 +366,12 @@ def test_another_stream_and_two_at_once(dtype):
 
 @BOTH
 @pytest.mark.parametrize("through_autograd", [False, True])
-def test_captured_and_replayed(through_autograd, dtype):
+@pytest.mark.parametrize("n", [1, 12, 400])
+def test_captured_and_replayed(n, through_autograd, dtype):
     """A captured loss with its gradients, replayed on other inputs with another number of kept rows, two graphs in
     turn. Outside autograd also while an eager graph of the same leaves lives."""
     from hffn_b200.losses import linear_cross_entropy, linear_cross_entropy_gradients
-    h, w, t = make(400, 128, 2000, dtype, seed=18, ignored=0.1)
+    h, w, t = make(n, 128, 2000, dtype, seed=18, ignored=0.1)
     h, w = h.requires_grad_(True), w.requires_grad_(True)
     eager = None if through_autograd else linear_cross_entropy(h, w, t)
 
@@ -389,7 +393,7 @@ def test_captured_and_replayed(through_autograd, dtype):
             outs.append(step(reduction))
         graphs.append(graph)
     for seed, ignored in ((19, 0.6), (20, 0.0), (21, 1.0)):
-        h2, w2, t2 = make(400, 128, 2000, dtype, seed=seed, ignored=ignored)
+        h2, w2, t2 = make(n, 128, 2000, dtype, seed=seed, ignored=ignored)
         with torch.no_grad():
             h.copy_(h2), w.copy_(w2), t.copy_(t2)
         for graph in graphs:
