@@ -28,8 +28,8 @@
 // entry (2048 x 1024 x 50304: 50 of 600 us). Sums: the tensor core's float32 accumulation truncates at every step, so
 // what ends in float32 (float32 gradients, losses) is summed in registers from accumulators of few steps each (chunk_of).
 //
-// Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 252 us, g 258 us, dh and dw 534 us (1.6 to 1.7
-// PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 204, 225 and 438 us (89, 80 and 93 %).
+// Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 258 us, g 263 us, dh and dw 546 us (1.57 to 1.67
+// PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 208, 236 and 447 us (90, 77 and 93 %).
 // Back to back for a second or more the card's power limit sets the rate: 1.42 PFLOP/s for 8192 x 2048 x 50304 logits,
 // what the library's plain product sustains.
 #include <cuda_fp16.h>
