@@ -158,18 +158,26 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
   return bits < 0x7f800000u ? bits : 0u;
 }
 
-__device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
-  hi = __float2half_rn(x);
-  lo = __float2half_rn(x - __half2float(hi));
+// Eight values as fp16 parts, 16 bytes each; two at a time, since the single conversions run at a quarter of the rate.
+__device__ __forceinline__ void split8(const float* x, uint4& hi, uint4& lo) {
+  uint32_t h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2 high = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
+    const float2 back = __half22float2(high);
+    const __half2 low = __floats2half2_rn(x[2 * j] - back.x, x[2 * j + 1] - back.y);
+    h[j] = *reinterpret_cast<const uint32_t*>(&high);
+    l[j] = *reinterpret_cast<const uint32_t*>(&low);
+  }
+  hi = make_uint4(h[0], h[1], h[2], h[3]);
+  lo = make_uint4(l[0], l[1], l[2], l[3]);
 }
 
-// Eight values as fp16 parts, 16 bytes each.
 __device__ __forceinline__ void store_parts(const float (&x)[8], __half* hi, __half* lo) {
-  __align__(16) __half h[8], l[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) split(x[j], h[j], l[j]);
-  *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(h);
-  *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(l);
+  uint4 h, l;
+  split8(x, h, l);
+  *reinterpret_cast<uint4*>(hi) = h;
+  *reinterpret_cast<uint4*>(lo) = l;
 }
 
 // ---- which rows are kept ------------------------------------------------------------------------------------------
@@ -617,8 +625,8 @@ struct RowEpilogue {
       if (EPI == kGrad) {
         sums = live ? e.s.sums[row] : make_float2(0.f, 1.f);
         lse2 = (sums.x + logf(sums.y)) * kLog2e;
-        sums.y = 1.f / sums.y;
         c = PARTS == 2 ? 16384.f : live && e.upstream.reduction == HFFN_REDUCE_NONE ? e.upstream.of(e.s, row, kept) : 1.f;
+        sums.y = c / sums.y;
       }
     }
   }
@@ -634,7 +642,7 @@ struct RowEpilogue {
   }
 
   __device__ __forceinline__ void columns(float (&v)[32], int col) {
-    if constexpr (EPI == kGradients || (PARTS == 2 && EPI == kGrad)) {
+    if constexpr (EPI == kGradients) {
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= factor;
     }
@@ -678,26 +686,26 @@ struct RowEpilogue {
     } else if constexpr (EPI == kGrad) {
       const int at = target - e.v0 - col;
       // float32: relative to the largest logit, whose difference is exact where p is large (an argument rounded at
-      // the size of the logit puts 1e-6 on p, and p - 1 may be small)
+      // the size of the logit puts 1e-6 on p, and p - 1 may be small); `factor` and c are powers of two
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        v[j] = PARTS == 2 ? exp2_fast((v[j] - sums.x) * kLog2e) * sums.y : exp2_fast(fmaf(v[j], kLog2e, -lse2));
+        v[j] = PARTS == 2 ? exp2_fast(fmaf(v[j], factor, -sums.x) * kLog2e) * sums.y
+                          : c * exp2_fast(fmaf(v[j], kLog2e, -lse2));
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (at == j) v[j] -= 1.f;
+          if (at == j) v[j] -= c;
       }
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] = live ? c * v[j] : 0.f;
+      for (int j = 0; j < 32; ++j) v[j] = live ? v[j] : 0.f;
       const int at_block = out.template begin<PARTS * kOutBytes / 2>();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if constexpr (PARTS == 2) {
-          __align__(16) __half hi[8], lo[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) split(v[8 * q + j], hi[j], lo[j]);
-          out.template put<64>(0, q, *reinterpret_cast<const uint4*>(hi));
-          out.template put<64>(kOutBytes / 2, q, *reinterpret_cast<const uint4*>(lo));
+          uint4 hi, lo;
+          split8(v + 8 * q, hi, lo);
+          out.template put<64>(0, q, hi);
+          out.template put<64>(kOutBytes / 2, q, lo);
         } else {
           out.template put<64>(at_block, q, pack_bf16(v + 8 * q));
         }
