@@ -23,8 +23,8 @@ namespace clip {
 
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;             // entries a block takes at a time
-// Blocks of one launch, the fastest of 4 to 16 per SM (582 M bfloat16 entries): the norm 213 us with 4 (265 with 8: its
-// float64 conversions share each SM's one slow pipe), the scaling 558 us with 16 (597 with 8).
+// Blocks of one launch, the fastest of 4 to 16 per SM (582 M bfloat16 entries): the norm 213 us with 4 (265 with 8), the
+// scaling 558 us with 16 (597 with 8).
 constexpr int kNormBlocks = 148 * 4, kScaleBlocks = 148 * 16;
 constexpr int kTableMax = 1000;          // 32 bytes each: within the 32764 bytes of kernel parameters
 constexpr int kMaxTensors = 64000;

@@ -39,10 +39,13 @@ def _check(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
 
 @lru_cache(maxsize=256)
 def _sizes(code: int, n: int, d: int, vocab: int) -> tuple[int, int, int]:
-    """Bytes of the state, the forward's and the backward's workspace."""
-    return (native.lib.hffn_linear_ce_state_bytes(code, n, d, vocab),
-            native.lib.hffn_linear_ce_forward_workspace(code, n, d, vocab),
-            native.lib.hffn_linear_ce_backward_workspace(code, n, d, vocab))
+    """Bytes of the state, the forward's and the backward's workspace; ValueError for sizes the kernels do not take."""
+    sizes = (native.lib.hffn_linear_ce_state_bytes(code, n, d, vocab),
+             native.lib.hffn_linear_ce_forward_workspace(code, n, d, vocab),
+             native.lib.hffn_linear_ce_backward_workspace(code, n, d, vocab))
+    if min(sizes) < 0:
+        native.check(native.HFFN_ERR_ARGUMENT, "linear cross entropy")
+    return sizes
 
 
 def _forward(hidden, weight, targets, ignore_index, reduction, for_backward=True):
@@ -114,7 +117,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     are the gradients. A target outside [0, vocabulary) that is not ``ignore_index`` makes its token's loss (and the
     sum and the mean) NaN and gives no gradient: it is found without a host synchronisation.
 
-    Arguments are checked before any launch (ValueError). One backward per forward result (no second derivatives)."""
+    Arguments are checked before any launch (ValueError). No second derivatives."""
     _check(hidden, weight, targets, reduction)
     rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):

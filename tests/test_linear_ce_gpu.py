@@ -521,6 +521,7 @@ def test_refusals():
                 lambda: linear_cross_entropy(h[:, :60], w[:, :60].contiguous(), t),
                 lambda: linear_cross_entropy(h[:, :56], w[:, :56], t),
                 lambda: linear_cross_entropy(h, torch.zeros(300 * 64 + 1, device="cuda")[1:].view(300, 64), t),
+                lambda: linear_cross_entropy(torch.zeros(20, 32776, device="cuda"), torch.zeros(3, 32776, device="cuda"), t),
                 lambda: linear_cross_entropy(h, w[:0], t),
                 lambda: linear_cross_entropy(h[:0], w, t[:0])):
         with pytest.raises(ValueError):

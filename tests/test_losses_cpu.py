@@ -17,6 +17,15 @@ def test_losses_refuse_bad_arguments():
             bad()
 
 
+def test_sizes_the_kernels_do_not_take():
+    from hffn_b200 import _native as n
+    from hffn_b200.losses import _sizes
+    assert min(_sizes(n.F32, 100, 64, 1000)) > 0
+    for n_tokens, d, vocab in ((100, 32776, 1000), (1 << 24, 64, 1 << 24), (100, 64, (1 << 24) + 1)):
+        with pytest.raises(ValueError):
+            _sizes(n.BF16, n_tokens, d, vocab)
+
+
 def test_linear_ce_entries_refuse_bad_arguments():
     from hffn_b200 import _native as n
     lib = n.lib
