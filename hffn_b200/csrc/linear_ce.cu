@@ -1176,7 +1176,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const T* hidden, int64
     if (v < vocab) {
       const float z = acc[0];
       if (v == target) picked[first + row] = z;
-      merge(top, sum, z, 1.f);
+      merge(top, sum, z, z == z ? 1.f : z);      // no maximum keeps a NaN: it stays in the sum
     }
   }
   shared[warp][lane] = make_float2(top, sum);

@@ -526,3 +526,19 @@ def test_refusals():
                 lambda: linear_cross_entropy(h[:0], w, t[:0])):
         with pytest.raises(ValueError):
             bad()
+
+
+@BOTH
+@pytest.mark.parametrize("n", [1, 2, 8, 16, 17])
+@pytest.mark.parametrize("row", [0, 1, 777, 5002])
+def test_a_head_row_that_is_not_a_number_reaches_every_loss(row, n, dtype):
+    """Whatever kernel the number of tokens takes, and whichever lane comes upon the row first."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(n, 64, 5003, dtype, seed=28)
+    w, t = w.clone(), torch.full_like(t, 5)
+    w[row, 9] = float("nan")
+    assert bool(torch.isnan(linear_cross_entropy(h, w, t, reduction="none")).all())
+    h.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    (dh,) = torch.autograd.grad(losses.sum(), h)
+    assert bool(torch.isnan(losses).all()) and bool(torch.isnan(dh).any(1).all())
