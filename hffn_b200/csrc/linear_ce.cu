@@ -5,6 +5,12 @@
 // without the [n, vocab] logits: the forward reduces each tile of logits to a maximum and a sum of exponentials per
 // row, and the backward recomputes the logits of one piece of the vocabulary at a time into g.
 //
+// The sums leave the target's own logit out, so that with the odds o = sum_{v != target} exp(z_v - z_target)
+//   loss = log(1 + o),   g_target = -c o / (1 + o),
+// both without a difference of nearly equal numbers where the target is well predicted (o small): lse - z and p - 1 would
+// leave of a loss of 1e-5 two digits, and p - 1 of logits summed once more in another order fewer. g_target is the
+// forward's; the other entries of g are as close, relative to themselves, as their logits are absolutely.
+//
 // Only kept rows exist for the products: rows whose target is ignored (or out of range) are left out when the hidden
 // states are gathered, so they cost nothing and whatever they hold (infinities, NaN) reaches no sum. How many are
 // kept is known on the device alone; every kernel reads it there, so a call can be captured and replayed.
@@ -71,6 +77,7 @@ struct State {
   int32_t* place_of;   // [n] the kept row of each input row; -1: left out
   int32_t* target;     // [n]
   float2* sums;        // [n] of each kept row the largest logit and the sum of exponentials relative to it
+  float* own;          // [n] p - 1 of its target
   void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts)
   void* head[2];       // [vocab, d] float32: the head's fp16 parts
   float* inverse;      // [vocab] float32, no backward: the inverse scale of each row of the head
@@ -117,6 +124,7 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   s.place_of = c.take<int32_t>(n_pad);
   s.target = c.take<int32_t>(n_pad);
   s.sums = c.take<float2>(n_pad);
+  s.own = c.take<float>(n_pad);
   for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
   if (dtype == HFFN_F32)
     for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
@@ -401,7 +409,7 @@ struct Args {
   int d, vocab;
   int v0, width;           // the piece of the vocabulary
   int64_t n_pad;
-  float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials
+  float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials, the target's left out
   float* picked;           // kStats: [n_pad] the target's logit
   Upstream upstream;
   const float* head_inverse;   // kStats, float32: of each row of the head (NULL: one scale for all)
@@ -664,7 +672,10 @@ struct RowEpilogue {
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (at == j) e.picked[row] = v[j] * factor;
+          if (at == j) {
+            e.picked[row] = v[j] * factor;
+            v[j] = -INFINITY;              // the sums are those of the others
+          }
       }
       // `factor` is a power of two, so it goes into the exponents' and the maximum's multiplications unrounded
       float most = v[0];
@@ -694,7 +705,7 @@ struct RowEpilogue {
       if (__any_sync(0xffffffffu, at >= 0 && at < 32)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
-          if (at == j) v[j] -= c;
+          if (at == j) v[j] = c * e.s.own[row];
       }
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = live ? v[j] : 0.f;
@@ -819,8 +830,9 @@ __device__ __forceinline__ bool load_stages(const Maps& maps, const Args& e, con
 // stage that cost (4 stages with the parts interleaved: dh of 46 tokens 1.2e-6 off, plain float32 sums 0.4e-6). Losses of
 // bfloat16 logits: 8 stages, 32 steps (8 x 511 tokens of 1024: 2.5e-7 off, plain sums 2.3e-7; 16 stages 5.2e-7 and no
 // faster; 4 stages 1.2e-7 but 8 to 15 % slower), and 4 where one row tile leaves the time to reading the head (few
-// losses average less, and that of a well predicted token is a small difference of logits). bfloat16 gradients are
-// rounded to 2^-8 afterwards and need none.
+// losses average less, and that of a well predicted token is a small difference of logits). bfloat16 gradients need none: an
+// error of a recomputed logit is one of p relative to itself, where g is rounded to 2^-8 of itself (p - 1 of the target,
+// where it would be more, is the forward's), and dh and dw are rounded to 2^-8 afterwards.
 template <int PARTS, int EPI>
 __device__ __forceinline__ int chunk_of(int kept) {
   return PARTS == 2 ? 2 : EPI == kStats ? (kept <= kTile ? 4 : 8) : 0;
@@ -1176,7 +1188,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const T* hidden, int64
     if (v < vocab) {
       const float z = acc[0];
       if (v == target) picked[first + row] = z;
-      merge(top, sum, z, z == z ? 1.f : z);      // no maximum keeps a NaN: it stays in the sum
+      else merge(top, sum, z, z == z ? 1.f : z);      // no maximum keeps a NaN: it stays in the sum
     }
   }
   shared[warp][lane] = make_float2(top, sum);
@@ -1194,7 +1206,8 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const T* hidden, int64
 }
 
 // ---- losses -------------------------------------------------------------------------------------------------------
-// lse and loss of the kept rows from the parts' maxima and sums: 32 rows a block, its 32 warps sharing the parts.
+// lse, loss and the target's p - 1 of the kept rows from their targets' logits and the parts' maxima and sums of the other
+// logits: 32 rows a block, its 32 warps sharing the parts.
 // The block that finishes last also adds up the losses where their sum or mean is asked for (float64, the same order
 // whichever block that is). The blocks after the `row_blocks` (bfloat16) zero the kept rows up to a whole stage of K of
 // the dw product.
@@ -1232,8 +1245,20 @@ __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* sta
     }
     const int mine = blockIdx.x * 32 + warp;
     if (lane == 0 && mine < kept) {
-      s.sums[mine] = v;
-      losses[s.row_of[mine]] = (v.x - picked[mine]) + logf(v.y);
+      const float z = picked[mine];
+      float of_row;
+      if (z >= v.x) {
+        const float odds = v.y * expf(v.x - z);
+        of_row = log1pf(odds) + (z - z);              // an infinite logit of the target: NaN
+        s.sums[mine] = make_float2(z, 1.f + odds);
+        s.own[mine] = -odds / (1.f + odds);
+      } else {
+        const float total = v.y + expf(z - v.x);
+        of_row = (v.x - z) + logf(total);
+        s.sums[mine] = make_float2(v.x, total);
+        s.own[mine] = -v.y / total;
+      }
+      losses[s.row_of[mine]] = of_row;
     }
   }
   if (reduction == HFFN_REDUCE_NONE) return;

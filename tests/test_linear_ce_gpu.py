@@ -542,3 +542,52 @@ def test_a_head_row_that_is_not_a_number_reaches_every_loss(row, n, dtype):
     losses = linear_cross_entropy(h, w, t, reduction="none")
     (dh,) = torch.autograd.grad(losses.sum(), h)
     assert bool(torch.isnan(losses).all()) and bool(torch.isnan(dh).any(1).all())
+
+
+@BOTH
+@pytest.mark.parametrize("n", [1, 12, 70])
+@pytest.mark.parametrize("size", [1e-3, 1e-4, 1e-5, 1e-7])
+def test_well_predicted_tokens(size, n, dtype):
+    """Losses of about `size` at a target's logit of 20 to 40: p - 1 is a small difference, of which every digit counts.
+    With the odds o = sum_{v != target} exp(z_v - z_target), loss = log(1 + o) and g_target = -o / (1 + o); every
+    difference of two logits is within 2 dz of the exact one (dz: of the largest logit's terms, since all of K may stay in
+    one accumulator in the backward), so o, the loss and every entry of g are within expm1(2 dz) of themselves, plus at
+    most 2^-18 of float32's own roundings (exponents' arguments of at most 64 are within 2^-18 of exact; sums and
+    functions are far closer), plus the storage of g and of the result."""
+    from hffn_b200.losses import linear_cross_entropy
+    d, v = 2048, 5000
+    g = torch.Generator(device="cuda").manual_seed(29)
+    w = (torch.randn(v, d, generator=g, device="cuda") / math.sqrt(d)).to(dtype)
+    t = torch.randint(0, v, (n,), generator=g, device="cuda")
+    noise = torch.randn(n, d, generator=g, device="cuda")
+    # about (log V + 1/2 - log size) / |w_t|^2 of the target's row: the odds come out near `size`
+    h = (noise + (math.log(v) + 0.5 - math.log(size)) * w[t].float()).to(dtype)
+    z = h.double() @ w.double().T
+    at = t[:, None]
+    difference = z - z.gather(1, at)
+    odds = difference.exp().scatter(1, at, 0.0).sum(1)
+    assert float(odds.max()) < 100 * size and float(z.gather(1, at).min()) > 8
+    fp32 = dtype == torch.float32
+    dz = (acc(d) + (2.0 ** -20 if fp32 else 0.0)) * (h.double().abs() @ w.double().abs().T).amax(1)
+    relative = torch.expm1(2 * dz) + 2.0 ** -18
+    exact = torch.log1p(odds)
+    h.requires_grad_(True), w.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    assert bool(((losses.detach().double() - exact).abs() <= relative * exact).all())
+    with torch.no_grad():
+        scored = linear_cross_entropy(h, w, t, reduction="none")
+    assert bool(((scored.double() - exact).abs() <= relative * exact).all())
+    dh, dw = torch.autograd.grad(losses.sum(), (h, w))
+    h, w = h.detach().double(), w.detach().double()
+    p = difference.exp() / (1 + odds)[:, None]
+    p.scatter_(1, at, -(odds / (1 + odds))[:, None])
+    held = 2.0 ** -39 if fp32 else 0.0
+    dg = p.abs() * (2 * relative + (2.0 ** -20 if fp32 else 2.0 ** -8))[:, None] + held
+    r = U if fp32 else 2.0 ** -8
+    split = 2.0 ** -20 if fp32 else 0.0
+    for got, want, bound in (
+            (dh, p @ w, dg @ w.abs() + (acc(v) + split) * (p.abs() @ w.abs())
+             + held * w.abs().amax() * p.abs().sum(1)[:, None]),
+            (dw, p.T @ h, dg.T @ h.abs() + (acc(n) + split) * (p.abs().T @ h.abs())
+             + held * h.abs().amax() * p.abs().sum(0)[:, None])):
+        assert bool(((got.double() - want).abs() <= 1.01 * (bound + r * want.abs()) + 1e-30).all())
