@@ -26,13 +26,14 @@
 // (the target's entry of a token that is not well predicted, the largest, is then close to -1, which is exact), and c
 // with it where they differ (a c h in bfloat16 beside it would round twice). float32: three fp16 products per product, of
 // operands held as two fp16 parts (hi = rn(x 2^e), lo = rn(x 2^e - hi); hi hi + hi lo + lo hi, the rest is below 2^-22),
-// 2^e one power of two per operand that brings its largest finite entry to [2^14, 2^15): entries down to 2^-17 of the
-// largest keep 22 bits, smaller ones are held to 2^-39 of it. One scale per operand, not per row, because each of h, w
-// and g is summed over its rows in one of the products. g holds 2^14 (p - [v = target]); c_t is applied in float32
-// afterwards (dh: per row; dw: one factor, or rows of h scaled by their c_t beforehand where they differ). A float32
-// forward without a backward takes a scale for each row of the head instead, which saves the pass that finds the largest
-// entry (2048 x 1024 x 50304: 50 of 600 us). Sums: the tensor core's float32 accumulation truncates at every step, so
-// what ends in float32 (float32 gradients, losses) is summed in registers from accumulators of few steps each (chunk_of).
+// 2^e a power of two that brings the largest finite entry to [2^14, 2^15): entries down to 2^-17 of the largest keep 22
+// bits, smaller ones are held to 2^-39 of it. For the logits every row of h and of w has a scale of its own, which is a
+// factor of its logits, so that no token or id takes bits from another, however large. dh sums over the rows of w, and dw
+// over those of h: there one scale has to serve the operand, whose parts the backward makes once more (rows_kernel: 59 us
+// of 2048 x 1024 x 50304). g holds 2^14 (p - [v = target]); c_t is applied in float32 afterwards (dh: per row; dw: one
+// factor, or rows of h scaled by their c_t beforehand where they differ). Sums: the tensor core's float32 accumulation
+// truncates at every step, so what ends in float32 (float32 gradients, losses) is summed in registers from accumulators of
+// few steps each (chunk_of).
 //
 // Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 258 us, g 263 us, dh and dw 546 us (1.57 to 1.67
 // PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 208, 236 and 447 us (90, 77 and 93 %).
@@ -72,15 +73,15 @@ __host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return (a + 
 struct State {
   int32_t* kept;       // [1] rows kept
   uint32_t* arrived;   // [1] blocks of the losses that are done
-  uint32_t* largest;   // [2] float32: bits of the largest finite |entry| of the kept rows and of the head
+  uint32_t* largest;   // [2] float32, backward: bits of the largest finite |entry| of the kept rows and of the head
   int32_t* row_of;     // [n] the input row of each kept row
   int32_t* place_of;   // [n] the kept row of each input row; -1: left out
   int32_t* target;     // [n]
   float2* sums;        // [n] of each kept row the largest logit and the sum of exponentials relative to it
   float* own;          // [n] p - 1 of its target
-  void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts)
-  void* head[2];       // [vocab, d] float32: the head's fp16 parts
-  float* inverse;      // [vocab] float32, no backward: the inverse scale of each row of the head
+  void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts, each row at a scale of its own)
+  void* head[2];       // [vocab, d] float32: the head's fp16 parts, each row at a scale of its own
+  float* hidden_inverse, *inverse;   // [n_pad], [vocab] float32: the inverse scales of those rows
   float* raw;          // [n, d] float32, few rows: the kept rows as they are (their parts are made in the backward)
   int64_t bytes;
 };
@@ -128,7 +129,10 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
   if (dtype == HFFN_F32)
     for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
-  if (dtype == HFFN_F32) s.inverse = c.take<float>(vocab);
+  if (dtype == HFFN_F32) {
+    s.hidden_inverse = c.take<float>(n_pad);
+    s.inverse = c.take<float>(vocab);
+  }
   if (dtype == HFFN_F32 && is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
   s.bytes = c.at;
   return s;
@@ -208,55 +212,27 @@ __device__ __forceinline__ int block_count(int mine, int* shared) {
   return total;
 }
 
+// Raises a largest magnitude by a whole warp's; most find it raised already, and spare the atomic.
 __device__ __forceinline__ void raise_largest(uint32_t* largest, uint32_t bits) {
   bits = __reduce_max_sync(0xffffffffu, bits);
-  if ((threadIdx.x & 31) == 0 && bits != 0) atomicMax(largest, bits);
+  if ((threadIdx.x & 31) == 0 && bits > *const_cast<volatile uint32_t*>(largest)) atomicMax(largest, bits);
 }
 
-// One block's share of the largest finite magnitude of an array (count a multiple of 4).
-__device__ __forceinline__ uint32_t largest_of(const float* array, int64_t count, int block, int blocks) {
-  const float4* from = reinterpret_cast<const float4*>(array);
-  const int64_t step = (int64_t)blocks * kGatherThreads;
-  uint32_t bits = 0;
-  auto raise = [&](float4 x) {
-    bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
-  };
-  int64_t i = (int64_t)block * kGatherThreads + threadIdx.x;
-  for (; i + 7 * step < count / 4; i += 8 * step) {
-    float4 x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = from[i + j * step];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) raise(x[j]);
-  }
-  for (; i < count / 4; i += step) raise(from[i]);
-  return bits;
-}
-
-// Blocks [0, gather): a block owns `span` consecutive input rows. It counts the kept rows before them (from the targets
-// alone, so that no block waits for another), places its own, and copies them (bfloat16) or raises the largest
-// magnitude by theirs (float32; a second kernel stores the parts). The other blocks (float32) raise the largest
-// magnitude of the head.
+// A block owns `span` consecutive input rows. It counts the kept rows before them (from the targets alone, so that no block
+// waits for another), places its own, and copies them (bfloat16; float32: a second kernel stores their parts).
 template <typename T>
-__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden, int64_t stride, const T* head,
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden, int64_t stride,
                                                                 const int64_t* targets, int64_t ignore, int n, int d,
-                                                                int vocab, int span, int gather, bool aligned,
-                                                                float* losses, State s) {
-  constexpr bool kF32 = sizeof(T) == 4;
+                                                                int vocab, int span, bool aligned, float* losses,
+                                                                State s) {
   __shared__ int shared[kGatherWarps];
   depend();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (kF32 && blockIdx.x >= gather) {
-    raise_largest(s.largest + 1, largest_of(reinterpret_cast<const float*>(head), (int64_t)vocab * d,
-                                            blockIdx.x - gather, gridDim.x - gather));
-    return;
-  }
   const int first = blockIdx.x * span, last = min(n, first + span);
   int mine = 0;
   for (int t = threadIdx.x; t < first; t += kGatherThreads) mine += is_kept(targets[t], ignore, vocab);
   int place = block_count(mine, shared);
   T* out = static_cast<T*>(s.hidden[0]);
-  uint32_t bits = 0;
   for (int base = first; base < last; base += 32) {      // every warp walks all rows and takes every eighth kept one
     const int t = base + lane;
     const int64_t target = t < last ? targets[t] : ignore;
@@ -273,12 +249,10 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
       }
     }
     int at = place;
-    for (unsigned left = mask; left; left &= left - 1, ++at) {
-      if ((at & (kGatherWarps - 1)) != warp) continue;
-      const T* from = hidden + (int64_t)(base + __ffs(left) - 1) * stride;
-      if constexpr (kF32) {
-        for (int i = lane; i < d; i += 32) bits = max(bits, finite_bits(from[i]));
-      } else {
+    if (sizeof(T) == 2)
+      for (unsigned left = mask; left; left &= left - 1, ++at) {
+        if ((at & (kGatherWarps - 1)) != warp) continue;
+        const T* from = hidden + (int64_t)(base + __ffs(left) - 1) * stride;
         T* to = out + (int64_t)at * d;
         if (aligned)
           for (int i = lane; i < d / 8; i += 32)
@@ -286,100 +260,136 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
         else
           for (int i = lane; i < d; i += 32) to[i] = from[i];
       }
-    }
     place += __popc(mask);
   }
-  if (kF32) raise_largest(s.largest, bits);
   if (last == n && threadIdx.x == 0) {
     *s.kept = place;
     *s.arrived = 0;
   }
 }
 
-// float32: the fp16 parts of the head and of the kept rows (from `hidden`, or from the state where `hidden` is NULL),
-// one warp a row; the kept rows are padded with zeros to a whole stage of K of the dw product. by_row: each row of the
-// head at a scale of its own.
-__global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t stride, bool aligned, const float* head,
-                                                    int d, int vocab, bool by_row, State s) {
-  depend();
-  const int lane = threadIdx.x & 31, kept = *s.kept;
-  int row = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const bool of_head = row < vocab;
-  if (!of_head) row -= vocab;
-  if (!of_head && row >= (int)round_up(kept, kBlockK)) return;
-  const bool zero = !of_head && row >= kept;
-  const float* from = of_head          ? head + (int64_t)row * d
-                      : zero           ? nullptr
-                      : hidden != NULL ? hidden + (int64_t)s.row_of[row] * stride
-                                       : s.raw + (int64_t)row * d;
-  uint32_t bits = 0;
-  if (of_head && by_row) {
-#pragma unroll 4
-    for (int i = 4 * lane; i < d; i += 128) {
-      const float4 x = *reinterpret_cast<const float4*>(from + i);
-      bits = max(max(bits, finite_bits(x.x)), max(finite_bits(x.y), max(finite_bits(x.z), finite_bits(x.w))));
-    }
-    bits = __reduce_max_sync(0xffffffffu, bits);
-    if (lane == 0) s.inverse[row] = power_of_two(-scale_exponent(bits));
+__device__ __forceinline__ void load8(const float* from, bool aligned, float (&x)[8]) {
+  if (aligned) {
+    *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from);
+    *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(from + 4);
   } else {
-    bits = s.largest[of_head];
-  }
-  const float scale = power_of_two(scale_exponent(bits));
-  __half* hi = static_cast<__half*>(of_head ? s.head[0] : s.hidden[0]) + (int64_t)row * d;
-  __half* lo = static_cast<__half*>(of_head ? s.head[1] : s.hidden[1]) + (int64_t)row * d;
-  for (int i = 8 * lane; i < d; i += 256) {
-    float x[8] = {};
-    if (zero) {
-    } else if (of_head || aligned) {
-      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from + i);
-      *reinterpret_cast<float4*>(x + 4) = *reinterpret_cast<const float4*>(from + i + 4);
-    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = from[i + j];
-    }
+    for (int j = 0; j < 8; ++j) x[j] = from[j];
+  }
+}
+
+// One warp: the fp16 parts of a row times `scale`, from value `first` on.
+__device__ __forceinline__ void split_row(const float* from, bool aligned, int first, int d, float scale, __half* hi,
+                                          __half* lo) {
+  for (int i = first + 8 * (threadIdx.x & 31); i < d; i += 256) {
+    float x[8];
+    load8(from + i, aligned, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] *= scale;
     store_parts(x, hi + i, lo + i);
   }
 }
 
-// float32, few rows, before the backward: the largest magnitudes of the kept rows (block 0) and of the head.
-__global__ void __launch_bounds__(kGatherThreads) measure_kernel(const float* head, int d, int vocab, State s) {
+// float32: the fp16 parts of the head and of the kept rows (from `hidden`, or from the state where `hidden` is NULL) for
+// the logits, one warp a row, each row at a scale of its own. for_backward: also the largest magnitudes of both.
+__global__ void __launch_bounds__(256) split_kernel(const float* hidden, int64_t stride, bool aligned, const float* head,
+                                                    int d, int vocab, bool for_backward, State s) {
   depend();
+  int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const bool of_head = row < vocab;
+  if (!of_head) row -= vocab;
+  if (!of_head && row >= *s.kept) return;
+  const float* from = of_head          ? head + (int64_t)row * d
+                      : hidden != NULL ? hidden + (int64_t)s.row_of[row] * stride
+                                       : s.raw + (int64_t)row * d;
+  aligned = aligned || of_head;
+  // the first kHeld values of a row stay in registers between the two passes over it (50304 rows of 1024: 61 us, 79 with
+  // a second read)
+  constexpr int kHeld = 4 * 256;
+  const int lane = threadIdx.x & 31;
+  float x[kHeld / 256][8];
   uint32_t bits = 0;
-  if (blockIdx.x == 0) {
-    for (int i = threadIdx.x; i < *s.kept * d; i += kGatherThreads) bits = max(bits, finite_bits(s.raw[i]));
-    raise_largest(s.largest, bits);
-  } else {
-    raise_largest(s.largest + 1, largest_of(head, (int64_t)vocab * d, blockIdx.x - 1, gridDim.x - 1));
+#pragma unroll
+  for (int k = 0; k < kHeld / 256; ++k) {
+    const int i = 256 * k + 8 * lane;
+    if (i < d) load8(from + i, aligned, x[k]);
   }
+#pragma unroll
+  for (int k = 0; k < kHeld / 256; ++k)
+    if (256 * k + 8 * lane < d)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bits = max(bits, finite_bits(x[k][j]));
+  for (int i = kHeld + lane; i < d; i += 32) bits = max(bits, finite_bits(from[i]));
+  bits = __reduce_max_sync(0xffffffffu, bits);
+  const int e = scale_exponent(bits);
+  const float scale = power_of_two(e);
+  if (lane == 0) (of_head ? s.inverse : s.hidden_inverse)[row] = power_of_two(-e);
+  if (for_backward) raise_largest(s.largest + of_head, bits);
+  const int64_t at = (int64_t)row * d;
+  __half* hi = static_cast<__half*>(of_head ? s.head[0] : s.hidden[0]) + at;
+  __half* lo = static_cast<__half*>(of_head ? s.head[1] : s.hidden[1]) + at;
+#pragma unroll
+  for (int k = 0; k < kHeld / 256; ++k) {
+    const int i = 256 * k + 8 * lane;
+    if (i >= d) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[k][j] *= scale;
+    store_parts(x[k], hi + i, lo + i);
+  }
+  split_row(from, aligned, kHeld, d, scale, hi, lo);
 }
 
-// float32, a gradient of its own for each token: rows c_t h_t of the kept rows, first their largest magnitude, then
-// their fp16 parts (padded with zeros to a whole stage of K).
-template <bool kStore>
-__global__ void __launch_bounds__(256) scaled_rows_kernel(State s, Upstream upstream, uint32_t* largest, __half* hi,
-                                                          __half* lo, int d) {
-  depend();
-  const int lane = threadIdx.x & 31, row = blockIdx.x * 8 + (threadIdx.x >> 5), kept = *s.kept;
-  if (row >= (kStore ? (int)round_up(kept, kBlockK) : kept)) return;
-  const float inverse = power_of_two(-scale_exponent(s.largest[0]));
-  const float c = row < kept ? upstream.of(s, row, kept) : 0.f;
-  const float scale = kStore ? power_of_two(scale_exponent(*largest)) : 1.f;
-  const __half* from_hi = static_cast<const __half*>(s.hidden[0]) + (int64_t)row * d;
-  const __half* from_lo = static_cast<const __half*>(s.hidden[1]) + (int64_t)row * d;
-  uint32_t bits = 0;
-  for (int i = 8 * lane; i < d; i += 256) {
-    float x[8];
+// float32: eight values of a kept row times c, from its parts.
+__device__ __forceinline__ void kept_values(const State& s, int row, int i, int d, float c, float (&x)[8]) {
+  const uint4 hi = *reinterpret_cast<const uint4*>(static_cast<const __half*>(s.hidden[0]) + (int64_t)row * d + i);
+  const uint4 lo = *reinterpret_cast<const uint4*>(static_cast<const __half*>(s.hidden[1]) + (int64_t)row * d + i);
+  const float inverse = s.hidden_inverse[row];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = row < kept ? c * ((__half2float(from_hi[i + j]) + __half2float(from_lo[i + j])) * inverse) : 0.f;
-      bits = max(bits, finite_bits(x[j]));
-      x[j] *= scale;
-    }
-    if (kStore) store_parts(x, hi + (int64_t)row * d + i, lo + (int64_t)row * d + i);
+  for (int j = 0; j < 8; ++j)
+    x[j] = c * ((__half2float(reinterpret_cast<const __half*>(&hi)[j]) +
+                 __half2float(reinterpret_cast<const __half*>(&lo)[j])) * inverse);
+}
+
+// float32, a gradient of its own for each token: the largest magnitude of the rows c_t h_t.
+__global__ void __launch_bounds__(256) scaled_largest_kernel(State s, Upstream upstream, uint32_t* largest, int d) {
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), kept = *s.kept;
+  if (row >= kept) return;
+  uint32_t bits = 0;
+  for (int i = 8 * (threadIdx.x & 31); i < d; i += 256) {
+    float x[8];
+    kept_values(s, row, i, d, upstream.of(s, row, kept), x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits = max(bits, finite_bits(x[j]));
   }
-  if (!kStore) raise_largest(largest, bits);
+  raise_largest(largest, bits);
+}
+
+// float32: the operands that dh and dw sum over, as fp16 parts at one scale each: `width` rows of the head, then of the
+// first `rows` kept rows h_t, or c_t h_t where each token has a gradient of its own (`each`), padded with zeros to a whole
+// stage of K. One warp a row.
+__global__ void __launch_bounds__(256) rows_kernel(const float* head, int width, __half* head_hi, __half* head_lo, State s,
+                                                   Upstream upstream, bool each, int rows,
+                                                   const uint32_t* rows_largest, __half* rows_hi, __half* rows_lo,
+                                                   int d) {
+  depend();
+  int row = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row < width) {
+    const int64_t at = (int64_t)row * d;
+    split_row(head + at, true, 0, d, power_of_two(scale_exponent(s.largest[1])), head_hi + at, head_lo + at);
+    return;
+  }
+  row -= width;
+  const int kept = *s.kept;
+  if (row >= min(rows, (int)round_up(kept, kBlockK))) return;
+  const float scale = power_of_two(scale_exponent(*rows_largest));
+  const float c = row < kept && each ? upstream.of(s, row, kept) : 1.f;
+  for (int i = 8 * (threadIdx.x & 31); i < d; i += 256) {
+    float x[8] = {};
+    if (row < kept) kept_values(s, row, i, d, c, x);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] *= scale;
+    store_parts(x, rows_hi + (int64_t)row * d + i, rows_lo + (int64_t)row * d + i);
+  }
 }
 
 // ---- products -----------------------------------------------------------------------------------------------------
@@ -412,7 +422,6 @@ struct Args {
   float2* stats;           // kStats: [2 per column tile][n_pad] maximum and sum of exponentials, the target's left out
   float* picked;           // kStats: [n_pad] the target's logit
   Upstream upstream;
-  const float* head_inverse;   // kStats, float32: of each row of the head (NULL: one scale for all)
   int add;                 // kGradients: dh adds to its slots (a later piece)
   const uint32_t* dw_rows_largest;   // float32: of the rows dw sums (h, or c h)
   int dw_upstream;                   // dw's rows lack their c, which is the same for all
@@ -600,7 +609,7 @@ struct RowEpilogue {
   int target;
   float factor;             // of the accumulators
   float top, sum;           // kStats
-  float4 inverse;           // kStats with a scale for each row of the head: of this lane's 4 of the warp's 128 columns
+  float4 inverse;           // logits of float32: the inverse scales of this lane's 4 of the warp's 128 columns
   float2 sums;              // kGrad
   float lse2, c;
 
@@ -618,17 +627,12 @@ struct RowEpilogue {
     } else {
       live = row < kept;
       target = live ? e.s.target[row] : -1;
-      if (PARTS == 2)
-        // within float32's range: logits that it cuts off there are zero or overflow anyway
-        factor = power_of_two(
-            max(-126, min(127, -scale_exponent(e.s.largest[0]) -
-                                   (EPI == kStats && e.head_inverse ? 0 : scale_exponent(e.s.largest[1])))));
+      if (PARTS == 2 && live) factor = e.s.hidden_inverse[row];
       top = -INFINITY;
       sum = 0.f;
-      if (PARTS == 2 && EPI == kStats && e.head_inverse) {
-        const int col = first_col + 4 * out.lane;       // the array is padded to a multiple of 64
-        inverse = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (col < e.vocab) inverse = __ldg(reinterpret_cast<const float4*>(e.head_inverse + col));
+      if (PARTS == 2) {
+        const int v = e.v0 + first_col + 4 * out.lane;       // the array is padded to a multiple of 64
+        inverse = v < e.vocab ? __ldg(reinterpret_cast<const float4*>(e.s.inverse + v)) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       if (EPI == kGrad) {
         sums = live ? e.s.sums[row] : make_float2(0.f, 1.f);
@@ -639,12 +643,19 @@ struct RowEpilogue {
     }
   }
 
-  // The sums are complete: the columns' scales where every lane reads them (nothing leaves through this memory here).
-  __device__ __forceinline__ void begin() {
-    if constexpr (PARTS == 2 && EPI == kStats) {
-      if (!e.head_inverse) return;
+  // The sums are complete. Logits of float32: their columns' scales, by way of shared memory where every lane reads them
+  // (once the stores of the last tile have been read out of it).
+  __device__ __forceinline__ void begin(float (&total)[128]) {
+    if constexpr (PARTS == 2 && EPI != kGradients) {
+      if (EPI == kGrad) out.template begin<kOutBytes>();
       __syncwarp();
       reinterpret_cast<float4*>(out.base)[out.lane] = inverse;
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 128; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(out.base + 4 * j);
+        total[j] *= x.x, total[j + 1] *= x.y, total[j + 2] *= x.z, total[j + 3] *= x.w;
+      }
       __syncwarp();
     }
   }
@@ -655,14 +666,6 @@ struct RowEpilogue {
       for (int j = 0; j < 32; ++j) v[j] *= factor;
     }
     if constexpr (EPI == kStats) {
-      if (PARTS == 2 && e.head_inverse) {
-        const float* scales = reinterpret_cast<const float*>(out.base) + (col & 127);
-#pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(scales + j);
-          v[j] *= x.x, v[j + 1] *= x.y, v[j + 2] *= x.z, v[j + 3] *= x.w;
-        }
-      }
       if (col + 32 > e.vocab) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
@@ -1015,7 +1018,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
           release_buffer();
         }
         if (!ok) break;
-        out.begin();
+        out.begin(total);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float v[32];
@@ -1465,7 +1468,8 @@ struct BackwardWork {
   void* g[2];
   float* slots;
   uint32_t* largest;      // float32, a gradient for each token: of c h
-  void* rows[2];          // and its fp16 parts
+  void* rows[2];          // float32, [n_pad, d]: the fp16 parts of the rows dw sums
+  void* head[2];          // float32, [piece_width, d]: those of the rows dh sums
   int64_t bytes;
 };
 
@@ -1478,6 +1482,7 @@ static BackwardWork backward_work(void* base, int dtype, int64_t n, int d, int v
   if (dtype == HFFN_F32) {
     w.largest = c.take<uint32_t>(1);
     for (int part = 0; part < 2; ++part) w.rows[part] = c.take<uint16_t>(n_pad * d);
+    for (int part = 0; part < 2; ++part) w.head[part] = c.take<uint16_t>((int64_t)piece_width(dtype, n, vocab) * d);
   }
   w.bytes = c.at;
   return w;
@@ -1490,10 +1495,6 @@ static int check(int dtype, int64_t n, int32_t d, int32_t vocab) {
   HFFN_REQUIRE(vocab >= 1 && vocab <= (1 << 24), "vocabulary %d out of range [1, 2^24]", vocab);
   HFFN_REQUIRE(ceil_div(n, kTile) * ceil_div(vocab, kTile) < (int64_t(1) << 30), "too many tokens times rows");
   return HFFN_OK;
-}
-
-static int measuring_blocks(int vocab, int d) {
-  return (int)std::min<int64_t>(148 * 8, ceil_div((int64_t)vocab * d, 4 * kGatherThreads));
 }
 
 template <typename T>
@@ -1523,13 +1524,11 @@ static int forward(const void* hidden, int64_t stride, const void* weight, const
     const int span = (int)std::max<int64_t>(16, ceil_div(n, 512)), gather = (int)ceil_div(n, span);
     const bool aligned = (reinterpret_cast<uintptr_t>(hidden) & 15) == 0 && stride * (int64_t)sizeof(T) % 16 == 0;
     if (PARTS == 2 && cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
-    const int measure = PARTS == 2 && for_backward ? measuring_blocks(vocab, d) : 0;
-    gather_kernel<T><<<gather + measure, kGatherThreads, 0, st>>>(rows, stride, head, targets, ignore, n, d, vocab, span,
-                                                                  gather, aligned, losses, e.s);
+    gather_kernel<T><<<gather, kGatherThreads, 0, st>>>(rows, stride, targets, ignore, n, d, vocab, span, aligned, losses,
+                                                        e.s);
     if constexpr (PARTS == 2)
-      launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, rows, stride, aligned,
-                                head, d, vocab, !for_backward, e.s);
-    if (PARTS == 2 && !for_backward) e.head_inverse = e.s.inverse;
+      launch_next<split_kernel>((unsigned)ceil_div((int64_t)vocab + n, 8), 256, 0, st, rows, stride, aligned, head, d,
+                                vocab, for_backward, e.s);
     Maps maps;
     HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
     HFFN_TRY((launch_products<PARTS, kStats>(maps, e, ceil_div(n, kTile) * ceil_div(vocab, kTile), true, st)));
@@ -1558,50 +1557,63 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
   bool prepared = false;             // a kernel of this call precedes the products
   if constexpr (PARTS == 2) {
     if (is_few(dtype, n, d)) {       // the forward has made no parts
-      const float* values = static_cast<const float*>(weight);
       if (cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
-      measure_kernel<<<1 + measuring_blocks(vocab, d), kGatherThreads, 0, st>>>(values, d, vocab, e.s);
-      launch_next<split_kernel>((unsigned)ceil_div(vocab + round_up(n, kBlockK), 8), 256, 0, st, (const float*)nullptr,
-                                (int64_t)0, true, values, d, vocab, false, e.s);
+      split_kernel<<<(unsigned)ceil_div((int64_t)vocab + n, 8), 256, 0, st>>>(
+          nullptr, 0, true, static_cast<const float*>(weight), d, vocab, true, e.s);
       prepared = true;
     }
   }
   const void* rows[2] = {e.s.hidden[0], e.s.hidden[1]};    // what dw sums
-  e.dw_rows_largest = e.s.largest;
   e.dw_upstream = reduction != HFFN_REDUCE_NONE;
-  if (PARTS == 2 && reduction == HFFN_REDUCE_NONE && grad_weight != nullptr) {
-    e.dw_rows_largest = w.largest;
+  const bool each = reduction == HFFN_REDUCE_NONE;
+  if (PARTS == 2 && grad_weight != nullptr) {
     rows[0] = w.rows[0];
     rows[1] = w.rows[1];
-    if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
-    const unsigned blocks = (unsigned)(e.n_pad / 8);
-    __half *hi = static_cast<__half*>(w.rows[0]), *lo = static_cast<__half*>(w.rows[1]);
-    scaled_rows_kernel<false><<<blocks, 256, 0, st>>>(e.s, e.upstream, w.largest, hi, lo, d);
-    launch_next<scaled_rows_kernel<true>>(blocks, 256, 0, st, e.s, e.upstream, w.largest, hi, lo, d);
-    prepared = true;
+    e.dw_rows_largest = each ? w.largest : e.s.largest;
+    if (each) {
+      if (cudaMemsetAsync(w.largest, 0, 4, st) != cudaSuccess) return launch_status("linear_ce");
+      scaled_largest_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, st>>>(e.s, e.upstream, w.largest, d);
+      prepared = true;
+    }
   }
-  const void* head[2] = {dtype == HFFN_F32 ? e.s.head[0] : weight, e.s.head[1]};
+  const void* head[2] = {PARTS == 2 ? w.head[0] : weight, w.head[1]};     // what dh sums
   const int64_t row_tiles = ceil_div(n, kTile), wide = ceil_div(d, kTile);
   for (int v0 = 0; v0 < vocab; v0 += width) {
     e.v0 = v0;
     e.width = std::min(width, vocab - v0);
     e.add = v0 > 0;
     const int64_t columns = ceil_div(e.width, kTile);
+    if constexpr (PARTS == 2) {
+      const float* from = static_cast<const float*>(weight) + (int64_t)v0 * d;
+      const int wide_rows = grad_hidden != nullptr ? e.width : 0;
+      const int kept_rows = grad_weight != nullptr && v0 == 0 ? (int)e.n_pad : 0;
+      const int64_t all = (int64_t)wide_rows + kept_rows;
+      __half *head_hi = static_cast<__half*>(w.head[0]), *head_lo = static_cast<__half*>(w.head[1]);
+      __half *rows_hi = static_cast<__half*>(w.rows[0]), *rows_lo = static_cast<__half*>(w.rows[1]);
+      const unsigned blocks = (unsigned)ceil_div(all, 8);
+      if (all > 0 && prepared)
+        launch_next<rows_kernel>(blocks, 256, 0, st, from, wide_rows, head_hi, head_lo, e.s, e.upstream, each,
+                                 kept_rows, e.dw_rows_largest, rows_hi, rows_lo, d);
+      else if (all > 0)
+        rows_kernel<<<blocks, 256, 0, st>>>(from, wide_rows, head_hi, head_lo, e.s, e.upstream, each, kept_rows,
+                                            e.dw_rows_largest, rows_hi, rows_lo, d);
+      prepared = prepared || all > 0;
+    }
     Maps maps;
     HFFN_TRY(logits_job(maps, e, dtype, weight, n, d, vocab));
     for (int part = 0; part < PARTS; ++part)
       HFFN_TRY(make_map(&maps.out[part], part_type(dtype), w.g[part], e.n_pad, width, width, 32, 32));
-    HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, v0 > 0 || prepared, st)));
+    HFFN_TRY((launch_products<PARTS, kGrad>(maps, e, row_tiles * columns, prepared, st)));
     e.jobs = 0;
     int64_t tiles = 0;
     if (grad_hidden != nullptr) {
       const int j = e.jobs++;
       for (int part = 0; part < PARTS; ++part) {
         HFFN_TRY(operand_map(&maps.a[j][part], dtype, w.g[part], e.n_pad, e.width, width, 128));
-        HFFN_TRY(operand_map(&maps.b[j][part], dtype, head[part], vocab, d, d, kBlockK));
+        HFFN_TRY(operand_map(&maps.b[j][part], dtype, head[part], PARTS == 2 ? e.width : vocab, d, d, kBlockK));
       }
       HFFN_TRY(make_map(&maps.out[0], CU_TENSOR_MAP_DATA_TYPE_FLOAT32, w.slots, splits * e.n_pad, d, d, 32, 32));
-      e.job[j] = {n, d, e.width, 0, splits, v0};
+      e.job[j] = {n, d, e.width, 0, splits, PARTS == 2 ? 0 : v0};
       tiles += row_tiles * wide * splits;
     }
     if (grad_weight != nullptr) {
@@ -1618,6 +1630,7 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
       tiles += columns * wide;
     }
     if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, true, st)));
+    prepared = true;
   }
   if (grad_hidden != nullptr)
     launch_next<scatter_kernel<T>>((unsigned)ceil_div(n, 8), 256, 0, st, e.s, (const float*)w.slots, splits, e.n_pad,

@@ -117,6 +117,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     are the gradients. A target outside [0, vocabulary) that is not ``ignore_index`` makes its token's loss (and the
     sum and the mean) NaN and gives no gradient: it is found without a host synchronisation.
 
+    Accuracy. bfloat16: products of the inputs as they are; the probabilities less the targets are held in bfloat16 (2^-8
+    of each) on their way into the gradients. float32: the operands of the products keep 22 bits (two fp16 parts), in the
+    losses whatever the sizes of the rows. In the gradients small terms beside large ones keep less: an entry of
+    ``weight`` in ``grad_hidden``, or of ``hidden`` (times its token's gradient, for ``reduction="none"``) in
+    ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to 2^-39: a row of ``grad_weight`` whose
+    id is nowhere more probable than 1e-9 is off by up to a thousandth of itself, and is 0 from about 1e-12 on.
+
     Arguments are checked before any launch (ValueError). No second derivatives."""
     _check(hidden, weight, targets, reduction)
     rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))

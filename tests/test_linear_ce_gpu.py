@@ -591,3 +591,49 @@ def test_well_predicted_tokens(size, n, dtype):
             (dw, p.T @ h, dg.T @ h.abs() + (acc(n) + split) * (p.abs().T @ h.abs())
              + held * h.abs().amax() * p.abs().sum(0)[:, None])):
         assert bool(((got.double() - want).abs() <= 1.01 * (bound + r * want.abs()) + 1e-30).all())
+
+
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e20, 3e38])
+@pytest.mark.parametrize("n", [20, 300])
+def test_a_huge_hidden_row_leaves_the_others_alone(n, size):
+    """float32: one kept row of any finite size changes nothing of the other tokens' losses and of their rows of
+    grad_hidden, scoring and training alike."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(n, 128, 900, torch.float32, seed=30)
+    others = torch.arange(n, device="cuda") != 7
+    huge = h.clone()
+    huge[7] = torch.sign(h[7]) * size * torch.rand(128, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")
+    expected = reference(h, w, t, others.float())
+    for hidden in (h, huge):
+        scored = linear_cross_entropy(hidden, w, t, reduction="none")
+        hidden = hidden.detach().requires_grad_(True)
+        losses = linear_cross_entropy(hidden, w, t, reduction="none")
+        (dh,) = torch.autograd.grad(losses, hidden, others.float())
+        for got in (scored, losses.detach()):
+            within(got[others], [x[others] for x in expected[0]], "losses")
+        within(dh[others], [x[others] for x in expected[1]], "grad_hidden")
+
+
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e20, -float(torch.finfo(torch.float32).min) / 2])
+@pytest.mark.parametrize("n", [5, 20, 300])
+def test_a_huge_head_row_leaves_the_losses_alone(n, size):
+    """float32: an id that its row puts far out of reach (its logits are of -`size`) changes no loss, scoring and training
+    alike, nor the other rows of grad_weight."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(n, 128, 900, torch.float32, seed=31)
+    h, w, t = h.clone(), w.clone(), torch.where(t == 400, 401, t)
+    h[:, 5] = 1.0 + h[:, 5].abs()
+    others = torch.arange(900, device="cuda") != 400
+    w[400] = 0
+    w[400, 5] = -1.0
+    w[400] *= size
+    rest = w[others].contiguous()
+    expected = reference(h, rest, t - (t > 400).long(), torch.ones(n, device="cuda"))
+    with torch.no_grad():
+        within(linear_cross_entropy(h, w, t, reduction="none"), expected[0], "scored losses")
+    w.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    (dw,) = torch.autograd.grad(losses.sum(), w)
+    within(losses.detach(), expected[0], "losses")
+    within(dw[others], expected[2], "grad_weight")
+    assert bool((dw[400] == 0).all())
