@@ -122,7 +122,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     losses whatever the sizes of the rows. In the gradients small terms beside large ones keep less: an entry of
     ``weight`` in ``grad_hidden``, or of ``hidden`` (times its token's gradient, for ``reduction="none"``) in
     ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to 2^-39: a row of ``grad_weight`` whose
-    id is nowhere more probable than 1e-9 is off by up to a thousandth of itself, and is 0 from about 1e-12 on.
+    id is nowhere more probable than 1e-9 is off by up to two thousandths of itself, and is 0 from about 1e-12 on.
 
     Arguments are checked before any launch (ValueError). No second derivatives."""
     _check(hidden, weight, targets, reduction)
