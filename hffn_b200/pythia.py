@@ -247,7 +247,7 @@ def train_step(model: nn.Module, optimizer, input_ids: torch.Tensor, labels: tor
     loss = causal_lm_loss(model, input_ids, labels, **inputs)
     loss.backward()
     others = [p.grad for p in model.parameters() if p.grad is not None]
-    norm = train.clip_grad_norm(float("inf") if max_norm is None else max_norm, others)
+    norm = train.clip_grad_norm(max_norm, others)
     optimizer.step()
     for index in range(len(train.steps)):
         train.adamw(index)

@@ -323,15 +323,18 @@ class HFFNTrainRuntime:
         """AdamW from the stored gradients (after a data-parallel exchange); the dense operands are rebuilt lazily."""
         self.adamw(index)
 
-    def clip_grad_norm(self, max_norm: float, tensors=(), layers=None) -> torch.Tensor:
+    def clip_grad_norm(self, max_norm: float | None, tensors=(), layers=None) -> torch.Tensor:
         """Clip the stored compact gradients of ``layers`` (indices; default all) together with ``tensors`` (the
         gradients of a model's other parameters) by their global norm, in place, before ``adamw``: every entry times
         ``min(1, max_norm / (norm + 1e-6))``. Returns the norm before it, a float32 scalar on the device
-        (``grad_clip.clip_grad_norm``; no host synchronisation). The steps that fuse AdamW into the backward (``step``,
+        (``grad_clip.clip_grad_norm``; no host synchronisation). ``max_norm`` None: the norm only, nothing is written,
+        whatever the gradients hold (``grad_clip.grad_norm``). The steps that fuse AdamW into the backward (``step``,
         ``step_mse``) apply their gradients unclipped."""
-        from .grad_clip import clip_grad_norm
+        from .grad_clip import clip_grad_norm, grad_norm
         layers = range(len(self._grads)) if layers is None else layers
         compact = [grad for index in layers for grad in self._grads[index].values()]
+        if max_norm is None:
+            return grad_norm([*compact, *tensors])
         return clip_grad_norm([*compact, *tensors], max_norm)
 
     # -- stacks of layers: every call keeps its own activations ---------------------------------------------------

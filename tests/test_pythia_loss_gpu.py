@@ -156,3 +156,21 @@ def test_refusals(tiny):
     with pytest.raises(ValueError):
         model.hffn_train.clip_grad_norm(1.0, [shared])                     # the same gradient twice
     assert copy.copy(model.hffn_train.steps) == [0, 0]
+
+
+def test_no_limit_writes_no_gradient(tiny):
+    """max_norm=None is the norm only: gradients that are not finite stay where they are, the others as they were."""
+    whole, parts = load(tiny), load(tiny)
+    ids, labels = batch(12)
+    for model in (whole, parts):
+        weight = model.gpt_neox.layers[0].attention.dense.weight
+        weight.register_hook(lambda g: g.index_put((torch.tensor(3, device="cuda"), torch.tensor(4, device="cuda")),
+                                                   torch.tensor(float("inf"), device="cuda")))
+    still = torch.optim.SGD(whole.parameters(), lr=0.0)
+    loss, norm = pythia.train_step(whole, still, ids, labels)
+    pythia.causal_lm_loss(parts, ids, labels).backward()
+    assert math.isinf(float(norm)) and math.isfinite(float(loss))
+    for a, b in zip(whole.parameters(), parts.parameters()):
+        assert torch.equal(a.grad, b.grad)
+    for a, b in zip(compact(whole), compact(parts)):
+        assert torch.equal(a, b)
