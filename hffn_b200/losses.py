@@ -10,6 +10,7 @@ from __future__ import annotations
 from functools import lru_cache
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _native as native
 from .runtime import DTYPES, MAX_TOKENS
@@ -35,6 +36,8 @@ def _check(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, re
         raise ValueError("weight must be contiguous and 16-byte aligned")
     if not 1 <= targets.numel() <= MAX_TOKENS:
         raise ValueError("unsupported token count")
+    if unpack_dual(hidden).tangent is not None or unpack_dual(weight).tangent is not None:
+        raise ValueError("forward-mode derivatives are not supported")
 
 
 @lru_cache(maxsize=256)
@@ -124,7 +127,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to 2^-39: a row of ``grad_weight`` whose
     id is nowhere more probable than 1e-9 is off by up to two thousandths of itself, and is 0 from about 1e-12 on.
 
-    Arguments are checked before any launch (ValueError). No second derivatives."""
+    Arguments are checked before any launch (ValueError). No second derivatives and none in forward mode: a tensor with a
+    tangent is refused."""
     _check(hidden, weight, targets, reduction)
     rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):

@@ -637,3 +637,22 @@ def test_a_huge_head_row_leaves_the_losses_alone(n, size):
     within(losses.detach(), expected[0], "losses")
     within(dw[others], expected[2], "grad_weight")
     assert bool((dw[400] == 0).all())
+
+
+@BOTH
+@pytest.mark.parametrize("of", ["hidden", "weight"])
+def test_forward_mode_derivatives_are_refused(of, dtype):
+    """A tangent is never dropped without a word, with or without gradients."""
+    import torch.autograd.forward_ad as forward_ad
+    from hffn_b200.losses import linear_cross_entropy, linear_cross_entropy_gradients
+    h, w, t = make(20, 64, 300, dtype)
+    plain = linear_cross_entropy(h, w, t)
+    for grads in (False, True):
+        with forward_ad.dual_level(), torch.set_grad_enabled(grads):
+            assert torch.equal(linear_cross_entropy(h, w, t), plain)            # no tangent: as ever
+            hh = forward_ad.make_dual(h, torch.ones_like(h)) if of == "hidden" else h
+            ww = forward_ad.make_dual(w, torch.ones_like(w)) if of == "weight" else w
+            with pytest.raises(ValueError):
+                linear_cross_entropy(hh, ww, t)
+            with pytest.raises(ValueError):
+                linear_cross_entropy_gradients(hh, ww, t)
