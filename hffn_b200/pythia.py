@@ -238,11 +238,14 @@ def train_step(model: nn.Module, optimizer, input_ids: torch.Tensor, labels: tor
                max_norm: float | None = None, **inputs) -> tuple[torch.Tensor, torch.Tensor]:
     """One training step of a ``load_pythia(..., trainable=True)`` model: ``causal_lm_loss``, backward, the gradients of
     the FFNs and of every other parameter clipped together to ``max_norm`` (None: their norm only), ``optimizer`` (over
-    the model's other parameters) and the FFNs' compact AdamW. Returns the loss of the parameters before the update and
+    the model's other parameters) and the FFNs' compact AdamW. Gradients of earlier calls are cleared first, the
+    optimizer's and the model's: a parameter that requires a gradient counts in the norm with this step's, whether or not
+    the optimizer holds it. Returns the loss of the parameters before the update and
     the gradients' norm before clipping, both scalars on the device; the host waits for nothing."""
     train = getattr(model, "hffn_train", None)
     if train is None:
         raise ValueError("train_step needs a model loaded with trainable=True")
+    model.zero_grad(set_to_none=True)
     optimizer.zero_grad(set_to_none=True)
     loss = causal_lm_loss(model, input_ids, labels, **inputs)
     loss.backward()

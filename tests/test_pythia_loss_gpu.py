@@ -174,3 +174,17 @@ def test_no_limit_writes_no_gradient(tiny):
         assert torch.equal(a.grad, b.grad)
     for a, b in zip(compact(whole), compact(parts)):
         assert torch.equal(a, b)
+
+
+def test_a_parameter_outside_the_optimizer_adds_up_nothing(tiny):
+    """Every step's gradients are that step's own, whatever the optimizer holds."""
+    model = load(tiny)
+    held = [p for name, p in model.named_parameters() if "embed" not in name]
+    optimizer = torch.optim.SGD(held, lr=0.0)
+    model.hffn_train.lr = 0.0
+    ids, labels = batch(13)
+    _, first = pythia.train_step(model, optimizer, ids, labels)
+    grads = [p.grad.clone() for p in model.parameters()]
+    _, second = pythia.train_step(model, optimizer, ids, labels)
+    assert torch.equal(first, second)
+    assert all(torch.equal(p.grad, g) for p, g in zip(model.parameters(), grads))
