@@ -67,7 +67,9 @@ class ShardedHFFNMLP(nn.Module):
 class TrainableHFFNMLP(nn.Module):
     """Replacement of ``block.mlp`` for training: the layer ``index`` of an ``HFFNTrainRuntime`` as a torch autograd
     function (``HFFNFunction``): gradients flow to the model's other parameters through gx, the FFN's compact
-    gradients stay in the training runtime (``model.hffn_train``), whose ``adamw`` updates them."""
+    gradients stay in the training runtime (``model.hffn_train``), whose ``adamw`` updates them. They are computed
+    whether or not anything before the FFN requires a gradient: with the model's other parameters frozen, the FFNs train.
+    """
 
     def __init__(self, train, index: int) -> None:
         super().__init__()
@@ -76,7 +78,10 @@ class TrainableHFFNMLP(nn.Module):
     def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
         from .train_runtime import HFFNFunction
         shape = hidden_states.shape
-        y = HFFNFunction.apply(hidden_states.reshape(-1, shape[-1]).contiguous(), self.train_runtime, self.index)
+        x = hidden_states.reshape(-1, shape[-1]).contiguous()
+        if torch.is_grad_enabled() and not x.requires_grad:      # only parameters that are frozen come before it
+            x = x.detach().requires_grad_(True)
+        y = HFFNFunction.apply(x, self.train_runtime, self.index)
         return y.view(shape)
 
 

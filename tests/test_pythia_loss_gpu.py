@@ -188,3 +188,21 @@ def test_a_parameter_outside_the_optimizer_adds_up_nothing(tiny):
     _, second = pythia.train_step(model, optimizer, ids, labels)
     assert torch.equal(first, second)
     assert all(torch.equal(p.grad, g) for p, g in zip(model.parameters(), grads))
+
+
+def test_ffns_below_frozen_parameters_get_their_gradients(tiny):
+    """An FFN whose input carries no gradient has gradients of its own all the same: none is left from an earlier step."""
+    whole, frozen = load(tiny), load(tiny)
+    ids, labels = batch(14)
+    frozen.requires_grad_(False)
+    frozen.embed_out.weight.requires_grad_(True)
+    for model in (whole, frozen):
+        for index in range(SMALL["num_hidden_layers"]):
+            for g in model.hffn_train.gradients(index).values():
+                g.fill_(7.0)
+    pythia.causal_lm_loss(whole, ids, labels).backward()
+    pythia.train_step(frozen, torch.optim.SGD([frozen.embed_out.weight], lr=0.0), ids, labels)
+    for a, b in zip(compact(frozen), compact(whole)):
+        assert torch.equal(a, b)
+    assert torch.equal(frozen.embed_out.weight.grad, whole.embed_out.weight.grad)
+    assert all(p.grad is None for name, p in frozen.named_parameters() if name != "embed_out.weight")
