@@ -80,9 +80,11 @@ struct State {
   float2* sums;        // [n] of each kept row the largest logit and the sum of exponentials relative to it
   float* own;          // [n] p - 1 of its target
   void* hidden[2];     // [n_pad, d] the kept rows (float32: their fp16 parts, each row at a scale of its own)
+  float* hidden_inverse;   // [n_pad] float32: the inverse scales of those rows
   void* head[2];       // [vocab, d] float32: the head's fp16 parts, each row at a scale of its own
-  float* hidden_inverse, *inverse;   // [n_pad], [vocab] float32: the inverse scales of those rows
-  float* raw;          // [n, d] float32, few rows: the kept rows as they are (their parts are made in the backward)
+  float* inverse;      // [vocab] float32: the inverse scales of those rows
+  float* raw;          // [n, d] float32, few rows: the kept rows as they are. Their parts and the head's, for which the
+                       // backward has room, are made there
   int64_t bytes;
 };
 
@@ -114,6 +116,11 @@ static bool is_few(int dtype, int64_t n, int d) {
   return n <= (dtype == HFFN_F32 ? 2 * kFewRows : 1) && (int64_t)few_rows(dtype, n) * d * 4 <= kFewBytes;
 }
 
+static void take_head(Carve& c, void* (&head)[2], float*& inverse, int d, int vocab) {
+  for (int part = 0; part < 2; ++part) head[part] = c.take<uint16_t>((int64_t)vocab * d);
+  inverse = c.take<float>(vocab);
+}
+
 static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   Carve c{static_cast<uint8_t*>(base)};
   const int64_t n_pad = round_up(n, kTile);
@@ -127,13 +134,11 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   s.sums = c.take<float2>(n_pad);
   s.own = c.take<float>(n_pad);
   for (int part = 0; part < (dtype == HFFN_F32 ? 2 : 1); ++part) s.hidden[part] = c.take<uint16_t>(n_pad * d);
-  if (dtype == HFFN_F32)
-    for (int part = 0; part < 2; ++part) s.head[part] = c.take<uint16_t>((int64_t)vocab * d);
   if (dtype == HFFN_F32) {
     s.hidden_inverse = c.take<float>(n_pad);
-    s.inverse = c.take<float>(vocab);
+    if (is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
+    else take_head(c, s.head, s.inverse, d, vocab);
   }
-  if (dtype == HFFN_F32 && is_few(dtype, n, d)) s.raw = c.take<float>(n * d);
   s.bytes = c.at;
   return s;
 }
@@ -1453,11 +1458,11 @@ struct ForwardWork {
   int64_t bytes;
 };
 
-static ForwardWork forward_work(void* base, int64_t n, int vocab) {
+static ForwardWork forward_work(void* base, int dtype, int64_t n, int d, int vocab) {
   Carve c{static_cast<uint8_t*>(base)};
   const int64_t n_pad = round_up(n, kTile);
   ForwardWork w;
-  w.stats = c.take<float2>(std::max<int64_t>(2 * ceil_div(vocab, kTile), kFewBlocks) * n_pad);
+  w.stats = c.take<float2>((is_few(dtype, n, d) ? kFewBlocks : 2 * ceil_div(vocab, kTile)) * n_pad);
   w.picked = c.take<float>(n_pad);
   w.losses = c.take<float>(n_pad);
   w.bytes = c.at;
@@ -1470,6 +1475,8 @@ struct BackwardWork {
   uint32_t* largest;      // float32, a gradient for each token: of c h
   void* rows[2];          // float32, [n_pad, d]: the fp16 parts of the rows dw sums
   void* head[2];          // float32, [piece_width, d]: those of the rows dh sums
+  void* logits_head[2];   // float32, few rows: the state's `head` and `inverse`
+  float* logits_inverse;
   int64_t bytes;
 };
 
@@ -1483,6 +1490,7 @@ static BackwardWork backward_work(void* base, int dtype, int64_t n, int d, int v
     w.largest = c.take<uint32_t>(1);
     for (int part = 0; part < 2; ++part) w.rows[part] = c.take<uint16_t>(n_pad * d);
     for (int part = 0; part < 2; ++part) w.head[part] = c.take<uint16_t>((int64_t)piece_width(dtype, n, vocab) * d);
+    if (is_few(dtype, n, d)) take_head(c, w.logits_head, w.logits_inverse, d, vocab);
   }
   w.bytes = c.at;
   return w;
@@ -1503,7 +1511,7 @@ static int forward(const void* hidden, int64_t stride, const void* weight, const
                    cudaStream_t st) {
   constexpr int PARTS = sizeof(T) / 2;
   constexpr int dtype = PARTS == 2 ? HFFN_F32 : HFFN_BF16;
-  const ForwardWork w = forward_work(work, n, vocab);
+  const ForwardWork w = forward_work(work, dtype, n, d, vocab);
   Args e = {};
   e.s = state_at(state, dtype, n, d, vocab);
   e.d = d;
@@ -1557,6 +1565,9 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
   bool prepared = false;             // a kernel of this call precedes the products
   if constexpr (PARTS == 2) {
     if (is_few(dtype, n, d)) {       // the forward has made no parts
+      e.s.head[0] = w.logits_head[0];
+      e.s.head[1] = w.logits_head[1];
+      e.s.inverse = w.logits_inverse;
       if (cudaMemsetAsync(e.s.largest, 0, 8, st) != cudaSuccess) return launch_status("linear_ce");
       split_kernel<<<(unsigned)ceil_div((int64_t)vocab + n, 8), 256, 0, st>>>(
           nullptr, 0, true, static_cast<const float*>(weight), d, vocab, true, e.s);
@@ -1667,7 +1678,7 @@ int64_t hffn_linear_ce_state_bytes(int dtype, int64_t n, int32_t d, int32_t voca
 
 int64_t hffn_linear_ce_forward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab) {
   if (ce::check(dtype, n, d, vocab) != HFFN_OK) return -1;
-  return ce::forward_work(nullptr, n, vocab).bytes;
+  return ce::forward_work(nullptr, dtype, n, d, vocab).bytes;
 }
 
 int64_t hffn_linear_ce_backward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab) {

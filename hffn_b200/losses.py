@@ -127,7 +127,11 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to 2^-39: a row of ``grad_weight`` whose
     id is nowhere more probable than 1e-9 is off by up to two thousandths of itself, and is 0 from about 1e-12 on.
 
-    Arguments are checked before any launch (ValueError). No second derivatives and none in forward mode: a tensor with a
+    Memory. What the backward needs is kept until then: the kept rows of ``hidden`` (in ``hidden``'s type) and, for float32
+    and more than 16 tokens, the head's two parts, as many bytes as ``weight`` (scoring allocates those for the call). The
+    backward works on about 256 MB of probabilities at a time.
+
+    Arguments are checked before any launch (ValueError); an empty batch is refused. No second derivatives and none in forward mode: a tensor with a
     tangent is refused."""
     _check(hidden, weight, targets, reduction)
     rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))

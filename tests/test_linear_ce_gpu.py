@@ -656,3 +656,18 @@ def test_forward_mode_derivatives_are_refused(of, dtype):
                 linear_cross_entropy(hh, ww, t)
             with pytest.raises(ValueError):
                 linear_cross_entropy_gradients(hh, ww, t)
+
+
+def test_one_token_takes_little_memory():
+    """float32, a few tokens: the head is read as it is, so nothing of its size is allocated for a loss, and nothing of it
+    is kept for the backward."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(4, 1024, 20000, torch.float32, seed=32)
+    linear_cross_entropy(h, w, t)
+    torch.cuda.synchronize()
+    for hidden in (h, h.detach().requires_grad_(True)):
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        loss = linear_cross_entropy(hidden, w, t)
+        assert torch.cuda.max_memory_allocated() - before < w.numel()
+        del loss

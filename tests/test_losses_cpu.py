@@ -83,3 +83,13 @@ def test_clip_refuses_host_tensors():
         grad_norm([torch.zeros(3)])
     with pytest.raises(ValueError):
         clip_grad_norm([torch.zeros(3)], 1.0)
+
+
+def test_workspaces_follow_the_path_taken():
+    """Statistics of the few-row kernel's blocks only for few rows; head parts only where the call makes them."""
+    from hffn_b200 import _native as n
+    lib = n.lib
+    assert lib.hffn_linear_ce_forward_workspace(n.BF16, 1 << 20, 64, 1024) < 100 << 20
+    assert lib.hffn_linear_ce_state_bytes(n.F32, 1, 2048, 50304) < 8 << 20
+    assert lib.hffn_linear_ce_state_bytes(n.F32, 17, 2048, 50304) >= 4 * 2048 * 50304
+    assert lib.hffn_linear_ce_backward_workspace(n.F32, 1, 2048, 50304) >= 4 * 2048 * 50304
