@@ -74,6 +74,7 @@ struct State {
   int32_t* kept;       // [1] rows kept
   uint32_t* arrived;   // [1] blocks of the losses that are done
   uint32_t* largest;   // [2] float32, backward: bits of the largest finite |entry| of the kept rows and of the head
+  int32_t* failed;     // [1] not 0: a wait of the call ran out, tiles are missing from its results, which become NaN
   int32_t* row_of;     // [n] the input row of each kept row
   int32_t* place_of;   // [n] the kept row of each input row; -1: left out
   int32_t* target;     // [n]
@@ -125,9 +126,10 @@ static State state_at(void* base, int dtype, int64_t n, int d, int vocab) {
   Carve c{static_cast<uint8_t*>(base)};
   const int64_t n_pad = round_up(n, kTile);
   State s = {};
-  s.kept = c.take<int32_t>(4);
+  s.kept = c.take<int32_t>(5);
   s.arrived = reinterpret_cast<uint32_t*>(s.kept + 1);
   s.largest = reinterpret_cast<uint32_t*>(s.kept + 2);
+  s.failed = s.kept + 4;
   s.row_of = c.take<int32_t>(n_pad);
   s.place_of = c.take<int32_t>(n_pad);
   s.target = c.take<int32_t>(n_pad);
@@ -270,6 +272,7 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(const T* hidden,
   if (last == n && threadIdx.x == 0) {
     *s.kept = place;
     *s.arrived = 0;
+    *s.failed = 0;
   }
 }
 
@@ -784,6 +787,13 @@ __device__ __forceinline__ bool elect_one() {
   return elected != 0;
 }
 
+// What the thread of a warp whose wait ran out leaves: the device's error code, the call's mark, the other warps' sign.
+__device__ __forceinline__ void give_up(const State& s, volatile int* abort_flag, int code) {
+  atomicCAS(&g_error, 0, code);
+  *reinterpret_cast<volatile int32_t*>(s.failed) = 1;
+  *abort_flag = 1;
+}
+
 // A bounded wait of a whole warp: every lane gets the same answer.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, kWaitNs));
@@ -949,8 +959,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
         ok = load_stages<PARTS, EPI, 0>(maps, e, t, rank, smem, full, empty, ring, abort_flag);
     }
     if (!ok && lane == 0) {
-      atomicCAS(&g_error, 0, kErrLoad);
-      *abort_flag = 1;
+      give_up(e.s, abort_flag, kErrLoad);
       // the loads in flight land within microseconds; nothing waits on them any more, so this SM gives them time
       const uint64_t start = global_ns();
       while (global_ns() - start < 10000000ull) {
@@ -972,8 +981,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
       }
       if (lane == 0) {
         if (!ok) {
-          atomicCAS(&g_error, 0, kErrProduct);
-          *abort_flag = 1;
+          give_up(e.s, abort_flag, kErrProduct);
         }
       }
       __syncwarp();
@@ -1052,8 +1060,7 @@ product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Args e
     }
     block.finish();
     if (!ok && lane == 0) {
-      atomicCAS(&g_error, 0, kErrEpilogue);
-      *abort_flag = 1;
+      give_up(e.s, abort_flag, kErrEpilogue);
     }
   }
   __syncwarp();
@@ -1129,6 +1136,7 @@ __global__ void __launch_bounds__(kFewThreads) few_kernel(const T* hidden, int64
       if (writes) {
         *s.kept = kept_rows;
         *s.arrived = 0;
+        *s.failed = 0;
       }
     }
   }
@@ -1266,6 +1274,10 @@ __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* sta
         s.sums[mine] = make_float2(v.x, total);
         s.own[mine] = -v.y / total;
       }
+      if (*s.failed) {
+        of_row = s.own[mine] = NAN;
+        s.sums[mine] = make_float2(0.f, NAN);
+      }
       losses[s.row_of[mine]] = of_row;
     }
   }
@@ -1291,17 +1303,24 @@ __global__ void __launch_bounds__(1024) losses_kernel(State s, const float2* sta
   }
 }
 
-// dh of each input row: the sum of its kept row's slots (in order), or zeros. One warp a row.
+// dh of each input row: the sum of its kept row's slots (in order), or zeros. One warp a row. After a wait that ran out:
+// NaN for the kept rows, and for all of dw (`weight_count` entries, none where it is not wanted).
 template <typename T>
 __global__ void __launch_bounds__(256) scatter_kernel(State s, const float* slots, int splits, int64_t n_pad,
-                                                      Upstream upstream, T* grad_hidden, int n, int d) {
+                                                      Upstream upstream, T* grad_hidden, T* grad_weight,
+                                                      int64_t weight_count, int n, int d) {
   depend();
   const int t = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (t >= n) return;
+  const bool failed = *s.failed != 0;
+  if (failed)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < weight_count; i += (int64_t)gridDim.x * 256)
+      grad_weight[i] = from_f<T>(NAN);
+  if (t >= n || grad_hidden == nullptr) return;
   const int at = s.place_of[t];
   float factor = 1.f;      // what g lacks
   if (at >= 0 && (sizeof(T) == 4 || upstream.reduction != HFFN_REDUCE_NONE)) factor = upstream.of(s, at, *s.kept);
   if (sizeof(T) == 4) factor *= power_of_two(-14 - scale_exponent(s.largest[1]));
+  if (failed && at >= 0) factor = NAN;
   for (int i = 4 * lane; i < d; i += 128) {
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     if (at >= 0)
@@ -1643,9 +1662,10 @@ static int backward(const void* weight, int reduction, const float* grad_loss, v
     if (tiles > 0) HFFN_TRY((launch_products<PARTS, kGradients>(maps, e, tiles, true, st)));
     prepared = true;
   }
-  if (grad_hidden != nullptr)
-    launch_next<scatter_kernel<T>>((unsigned)ceil_div(n, 8), 256, 0, st, e.s, (const float*)w.slots, splits, e.n_pad,
-                                   e.upstream, static_cast<T*>(grad_hidden), n, d);
+  launch_next<scatter_kernel<T>>(grad_hidden != nullptr ? (unsigned)ceil_div(n, 8) : 1u, 256, 0, st, e.s,
+                                 (const float*)w.slots, splits, e.n_pad, e.upstream, static_cast<T*>(grad_hidden),
+                                 static_cast<T*>(grad_weight), grad_weight != nullptr ? (int64_t)vocab * d : (int64_t)0, n,
+                                 d);
   return launch_status("linear_ce_backward");
 }
 

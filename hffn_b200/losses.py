@@ -163,8 +163,8 @@ def linear_cross_entropy_gradients(hidden: torch.Tensor, weight: torch.Tensor, t
 
 
 def device_errors(device=None) -> int:
-    """The error flag of the loss's kernels on ``device`` (0: none; the code of a wait that ran out otherwise).
-    Synchronises."""
+    """The error flag of the loss's kernels on ``device`` (0: none; the code of a wait that ran out otherwise; the losses
+    or gradients of the call it ran out in are NaN). Synchronises."""
     flag = native.ctypes.c_int32(0)
     with torch.cuda.device(device):
         native.check(native.lib.hffn_linear_ce_error(native.ctypes.byref(flag), 0), "hffn_linear_ce_error")

@@ -385,7 +385,7 @@ int hffn_linear_ce_backward(int dtype, const void* weight, int reduction, const 
                             void* stream);
 
 /* The error flag of those kernels on the current device: 0, or the code of the first bounded wait that ran out (401, 402,
- * 403). Synchronous; clear != 0 resets it. */
+ * 403). Synchronous; clear != 0 resets it. The losses, or the gradients, of the call whose wait ran out are NaN. */
 int hffn_linear_ce_error(int32_t* value, int clear);
 
 /* The 2-norm over every entry of `count` tensors (no counterpart in the reference): tensors[i] holds numel[i] entries of

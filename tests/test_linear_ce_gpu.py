@@ -671,3 +671,22 @@ def test_one_token_takes_little_memory():
         loss = linear_cross_entropy(hidden, w, t)
         assert torch.cuda.max_memory_allocated() - before < w.numel()
         del loss
+
+
+@BOTH
+@pytest.mark.parametrize("wanted", [(True, True), (True, False), (False, True)])
+def test_no_gradient_from_a_wait_that_ran_out(wanted, dtype):
+    """A kernel whose wait runs out marks its call's state and leaves its tiles; the gradients are then NaN, not what the
+    tiles hold. The mark (the fifth word of the state) is set by hand here."""
+    from hffn_b200.losses import _backward, _forward
+    h, w, t = make(90, 64, 700, dtype, seed=33, ignored=0.2)
+    loss, state = _forward(h, w, t, IGNORE, "mean")
+    c = torch.ones_like(loss)
+    assert all(x is None or bool(torch.isfinite(x).all()) for x in _backward(w, state, 90, "mean", c, *wanted))
+    state[16:20].view(torch.int32).fill_(1)
+    dh, dw = _backward(w, state, 90, "mean", c, *wanted)
+    assert (dh is not None, dw is not None) == wanted
+    assert dh is None or torch.equal(torch.isnan(dh).all(1), t != IGNORE) and bool((dh[t == IGNORE] == 0).all())
+    assert dw is None or bool(torch.isnan(dw).all())
+    again, state = _forward(h, w, t, IGNORE, "mean")
+    assert torch.equal(again, loss) and bool(torch.isfinite(_backward(w, state, 90, "mean", c)[1]).all())
