@@ -35,8 +35,10 @@
 // truncates at every step, so what ends in float32 (float32 gradients, losses) is summed in registers from accumulators of
 // few steps each (chunk_of).
 //
-// Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 258 us, g 263 us, dh and dw 546 us (1.57 to 1.67
-// PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 208, 236 and 447 us (90, 77 and 93 %).
+// Measured (ncu, products alone): bfloat16 8192 x 2048 x 12800 logits 261 us, g 266 us, dh and dw 546 us (1.57 to 1.65
+// PFLOP/s, 96 to 97 % of the tensor pipe's cycles); float32 2048 x 1024 x 25344 218, 245 and 449 us (86, 74 and 93 %).
+// The kernels that sum in registers (all float32 ones, bfloat16 logits) use all 168 registers that 320 threads leave, and
+// spill 72 to 200 bytes a thread.
 // Back to back for a second or more the card's power limit sets the rate: 1.42 PFLOP/s for 8192 x 2048 x 50304 logits,
 // what the library's plain product sustains.
 #include <cuda_fp16.h>
@@ -102,9 +104,10 @@ struct Carve {
 
 // Few rows: their logits are computed on the CUDA cores, straight from the head (few_kernel), where that is faster than
 // the tensor cores' tiles. float32: up to 16 rows, in passes of 8, since it spares making the head's fp16 parts (a pass
-// of reads and one of writes before the products): d 1024, vocabulary 50304, whole calls: 47, 82 and 125 us for 4, 8 and
-// 16 rows against 149; 32 rows would take 228. bfloat16: one row (31 us against 36; two rows 42). The rows have to fit
-// the kernel's shared memory.
+// of reads and one of writes before the products): vocabulary 50304, whole calls, 4, 8 and 16 rows here against 17 in
+// tiles: d 512 31, 50 and 74 us against 79, d 1024 50, 80 and 122 against 131, d 2048 91, 140 and 219 against 245; 32 rows
+// of 1024 would take 228. bfloat16: one row against two in tiles: 23 us against 24, 32 against 37 and 51 against 58 (two
+// rows of 1024 here: 42). The rows have to fit the kernel's shared memory.
 constexpr int kFewRows = 8, kFewThreads = 256, kFewWarps = kFewThreads / 32;
 constexpr int64_t kFewBytes = 96 << 10;
 
@@ -1459,7 +1462,7 @@ static int logits_job(Maps& maps, Args& e, int dtype, const void* weight, int64_
   return HFFN_OK;
 }
 
-constexpr int kFewBlocks = 148 * 3;    // of the few-row kernel: 24 warps an SM
+constexpr int kFewBlocks = 148 * 3;    // of the few-row kernel: 24 warps an SM (8 float32 rows: 16, its registers allow two)
 
 template <typename T, int ROWS, int BATCH>
 static int launch_few(const T* hidden, int64_t stride, const T* head, const int64_t* targets, int64_t ignore, int n,

@@ -66,7 +66,8 @@ def _buffers(tensors: _List):
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm over every entry of ``tensors`` (one or many, float32 / bfloat16, dense, on one CUDA device): a float32
-    scalar on that device, computed in float64 and rounded once. An empty list has norm 0 (on the current device)."""
+    scalar on that device, computed in float64 and rounded once. An empty list has norm 0 (on the current device). Outside
+    autograd: the norm carries no derivative, whatever the tensors require."""
     tensors = _List(tensors, "tensors")
     norm, work = _buffers(tensors)
     with native.on_device(tensors.device):
@@ -83,7 +84,8 @@ def clip_grad_norm(tensors, max_norm: float, out=None) -> torch.Tensor:
     In place, or into ``out``: one tensor for each (float32 or bfloat16, e.g. an optimizer's float32 buffers for bfloat16
     gradients), contiguous with as many entries, or of the same shape and strides. The scaled values are computed in
     float32 and rounded once to the output's type.
-    With a norm that is infinite or NaN the factor is 0 or NaN, as with ``torch.nn.utils.clip_grad_norm_``.
+    With a norm that is infinite or NaN the factor is 0 or NaN, as with ``torch.nn.utils.clip_grad_norm_`` (an infinite
+    norm under an infinite ``max_norm``: NaN; for the norm alone there is ``grad_norm``).
     Refused (ValueError): tensors that share memory with one that is written, an output that overlaps another tensor's
     input, a negative ``max_norm``."""
     tensors = _List(tensors, "tensors")

@@ -120,19 +120,22 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     are the gradients. A target outside [0, vocabulary) that is not ``ignore_index`` makes its token's loss (and the
     sum and the mean) NaN and gives no gradient: it is found without a host synchronisation.
 
-    Accuracy. bfloat16: products of the inputs as they are; the probabilities less the targets are held in bfloat16 (2^-8
-    of each) on their way into the gradients. float32: the operands of the products keep 22 bits (two fp16 parts), in the
-    losses whatever the sizes of the rows. In the gradients small terms beside large ones keep less: an entry of
-    ``weight`` in ``grad_hidden``, or of ``hidden`` (times its token's gradient, for ``reduction="none"``) in
-    ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to 2^-39: a row of ``grad_weight`` whose
-    id is nowhere more probable than 1e-9 is off by up to two thousandths of itself, and is 0 from about 1e-12 on.
+    Accuracy. bfloat16: products of the inputs as they are; the probabilities less the targets (``reduction="none"``: times
+    the gradient of the token's loss) are held in bfloat16 (2^-8 of each) on their way into the gradients. float32: the
+    operands of the products are held as two fp16 parts. In the losses a row's entries keep 22 bits down to 2^-17 of its
+    largest and are held to 2^-39 of that below, whatever the other rows hold. The gradients sum over rows, and there small
+    terms beside large ones keep less: an entry of ``weight`` in ``grad_hidden``, or of ``hidden`` (times its token's
+    gradient, for ``reduction="none"``) in ``grad_weight``, is held to 2^-39 of that tensor's largest, and a probability to
+    2^-39: a row of ``grad_weight`` whose id is nowhere more probable than 1e-9 is off by up to two thousandths of itself,
+    and is 0 from about 1e-12 on. A NaN or infinity of ``hidden`` stays with its token in the losses and ``grad_hidden``,
+    one of ``weight`` reaches all.
 
     Memory. What the backward needs is kept until then: the kept rows of ``hidden`` (in ``hidden``'s type) and, for float32
     and more than 16 tokens, the head's two parts, as many bytes as ``weight`` (scoring allocates those for the call). The
     backward works on about 256 MB of probabilities at a time.
 
-    Arguments are checked before any launch (ValueError); an empty batch is refused. No second derivatives and none in forward mode: a tensor with a
-    tangent is refused."""
+    Arguments are checked before any launch (ValueError); an empty batch is refused. No second derivatives, and none in
+    forward mode: a tensor with a tangent is refused."""
     _check(hidden, weight, targets, reduction)
     rows, flat = (hidden, targets) if hidden.dim() == 2 else (hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1))
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):

@@ -367,8 +367,8 @@ int hffn_train_step_tc(const hffn_layer* layer, const hffn_dense* dense, const h
  * The logits are never stored. A row whose target is ignore_index has loss 0 and takes no part; its hidden state is not
  * read into any sum. A row whose target is otherwise outside [0, vocab) has loss NaN and no gradient. reduction NONE:
  * loss [n] float32; MEAN: *loss = the sum over the kept rows / max(1, kept rows); SUM. d: a multiple of 8.
- * state: hffn_linear_ce_state_bytes, kept for the backward (for_backward 0: no backward will read it); work: hffn_linear_ce_forward_workspace bytes (16-byte
- * aligned, as weight). */
+ * state: hffn_linear_ce_state_bytes, kept for the backward (for_backward 0: no backward will read it); work:
+ * hffn_linear_ce_forward_workspace bytes (16-byte aligned, as weight). */
 int64_t hffn_linear_ce_state_bytes(int dtype, int64_t n, int32_t d, int32_t vocab);
 int64_t hffn_linear_ce_forward_workspace(int dtype, int64_t n, int32_t d, int32_t vocab);
 int hffn_linear_ce_forward(int dtype, const void* hidden, int64_t hidden_stride, const void* weight,
