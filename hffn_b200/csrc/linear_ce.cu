@@ -619,6 +619,8 @@ struct RowEpilogue {
   bool live;                // the row exists
   int target;
   float factor;             // of the accumulators
+  float below;              // logits of float32: the part of it at most 1, applied before the columns' scales, so that
+                            // ordinary logits of a tiny and a huge row do not overflow on the way
   float top, sum;           // kStats
   float4 inverse;           // logits of float32: the inverse scales of this lane's 4 of the warp's 128 columns
   float2 sums;              // kGrad
@@ -638,7 +640,11 @@ struct RowEpilogue {
     } else {
       live = row < kept;
       target = live ? e.s.target[row] : -1;
-      if (PARTS == 2 && live) factor = e.s.hidden_inverse[row];
+      if (PARTS == 2) {
+        const float inverse_row = live ? e.s.hidden_inverse[row] : 1.f;
+        below = fminf(inverse_row, 1.f);
+        factor = fmaxf(inverse_row, 1.f);
+      }
       top = -INFINITY;
       sum = 0.f;
       if (PARTS == 2) {
@@ -665,7 +671,10 @@ struct RowEpilogue {
 #pragma unroll
       for (int j = 0; j < 128; j += 4) {
         const float4 x = *reinterpret_cast<const float4*>(out.base + 4 * j);
-        total[j] *= x.x, total[j + 1] *= x.y, total[j + 2] *= x.z, total[j + 3] *= x.w;
+        total[j] = total[j] * below * x.x;
+        total[j + 1] = total[j + 1] * below * x.y;
+        total[j + 2] = total[j + 2] * below * x.z;
+        total[j + 3] = total[j + 3] * below * x.w;
       }
       __syncwarp();
     }

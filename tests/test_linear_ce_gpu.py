@@ -690,3 +690,31 @@ def test_no_gradient_from_a_wait_that_ran_out(wanted, dtype):
     assert dw is None or bool(torch.isnan(dw).all())
     again, state = _forward(h, w, t, IGNORE, "mean")
     assert torch.equal(again, loss) and bool(torch.isfinite(_backward(w, state, 90, "mean", c)[1]).all())
+
+
+@BOTH
+@pytest.mark.parametrize("h_size,w_size", [(1e-37, 1e36), (1e36, 1e-37), (1e-30, 1e35), (1e35, 1e-30)])
+def test_operands_at_the_ends_of_float32(h_size, w_size, dtype):
+    """Ordinary logits of operands whose own scales leave float32 when either is applied before the other."""
+    from hffn_b200.losses import linear_cross_entropy
+    h, w, t = make(60, 128, 700, dtype, seed=34)
+    h, w = (h.float() * h_size).to(dtype), (w.float() * w_size).to(dtype)
+    h64, w64 = h.double(), w.double()
+    z = h64 @ w64.T
+    # an entry at 2^-126 and below keeps fewer bits than 22: a scale is at most 2^110, which leaves it to 2^-25 / 2^110
+    held = 2.0 ** -135 if dtype == torch.float32 else 0.0
+    dz = ((acc(128) + 2.0 ** -20) * (h64.abs() @ w64.abs().T) + held * w64.abs().sum(1) + held * h64.abs().sum(1)[:, None])
+    e = 2 * dz.amax(1) + 8 * U * (z.abs().amax(1) + 1 + math.log(700))
+    exact = torch.logsumexp(z, 1) - z.gather(1, t[:, None]).squeeze(1)
+    bound = e + 2 * U * (z.abs().amax(1) * 2 + math.log(700))
+    with torch.no_grad():
+        within(linear_cross_entropy(h, w, t, reduction="none"), (exact, bound), "scored losses")
+    h.requires_grad_(True)
+    losses = linear_cross_entropy(h, w, t, reduction="none")
+    within(losses.detach(), (exact, bound), "losses")
+    (dh,) = torch.autograd.grad(losses.sum(), h)
+    p = torch.softmax(z, 1).scatter_add(1, t[:, None], torch.full((60, 1), -1.0, dtype=torch.float64, device="cuda"))
+    r = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -20
+    size = p.abs() @ w64.abs()
+    limit = size * (2 * r + 2 * float(torch.expm1(e).max()) + acc(700)) + 2.0 ** -38 * w64.abs().sum(0)
+    assert bool(((dh.double() - p @ w64).abs() <= 1.01 * limit + 1e-37).all())
